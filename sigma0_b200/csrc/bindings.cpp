@@ -7,6 +7,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <algorithm>
 #include <cstdlib>
+#include <string>
 #include <vector>
 
 #include "launchers.h"
@@ -757,6 +758,214 @@ int64_t tp_gemm_allreduce(at::Tensor A, at::Tensor Bt, std::vector<int64_t> recv
   return tp_gemm_allreduce_launch(a, num_sms(A), stream());
 }
 
+// ---- decoding over a key / value cache ----------------------------------------------------------
+// numbers in the messages below go through this: inserting an integer into a stream here crashes where the
+// compiler's C++ library is not the one that torch was built with
+static std::string str(int64_t n) { return std::to_string(n); }
+
+static int kv_dtype(const at::Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return 0;
+    case at::kHalf: return 1;
+    case at::kBFloat16: return 2;
+    default: TORCH_CHECK(false, name, " must be float32, float16 or bfloat16"); return -1;
+  }
+}
+static void kv_ints(const at::Tensor& t, const char* name, int64_t n, const at::Device& dev) {
+  TORCH_CHECK(t.device() == dev && t.scalar_type() == at::kInt && t.is_contiguous() && t.numel() == n, name,
+              ": ", str(n), " int32 values on the cache's device");
+}
+// [.., B, nkv, S] float32 or int32 with contiguous slots
+static void kv_slots(const at::Tensor& t, const char* name, at::ScalarType dt, const at::Tensor& kc) {
+  TORCH_CHECK(t.device() == kc.device() && t.scalar_type() == dt, name, dt == at::kFloat ? " must be float32" : " must be int32",
+              " on the cache's device");
+  TORCH_CHECK(t.sizes() == kc.sizes().slice(0, kc.dim() - 1) && (t.stride(-1) == 1 || t.size(-1) <= 1), name,
+              " must have the cache's shape without the head dimension, slots contiguous");
+}
+static void kv_caches(const at::Tensor& kc, const at::Tensor& vc, int64_t dim) {
+  TORCH_CHECK(kc.is_cuda() && vc.device() == kc.device(), "the caches must be CUDA tensors of one device");
+  kv_dtype(kc, "k_cache");
+  TORCH_CHECK(kc.scalar_type() == vc.scalar_type(), "the caches must have one dtype");
+  TORCH_CHECK(kc.dim() == dim && kc.sizes() == vc.sizes(), "the caches must have one shape [",
+              dim == 5 ? "layers, " : "", "B, kv heads, slots, head dim]");
+  TORCH_CHECK(kc.stride(-1) == 1 && vc.stride(-1) == 1, "the caches' head dimension must be contiguous");
+  TORCH_CHECK(kc.size(-2) < (int64_t)1 << 30 && kc.size(-1) >= 1, "cache too long");
+}
+
+at::Tensor kv_attn(at::Tensor q, at::Tensor kn, at::Tensor vn, at::Tensor kc, at::Tensor vc, at::Tensor lengths,
+                   c10::optional<at::Tensor> mask, double scale, c10::optional<at::Tensor> weight,
+                   c10::optional<at::Tensor> positions, c10::optional<at::Tensor> seen) {
+  kv_caches(kc, vc, 4);
+  const auto dev = kc.device();
+  const int dt = kv_dtype(kc, "k_cache");
+  const int64_t B = kc.size(0), nkv = kc.size(1), S = kc.size(2), hd = kc.size(3);
+  TORCH_CHECK(q.dim() == 4 && kn.dim() == 4 && kn.sizes() == vn.sizes(), "q [B, T, heads, hd], k_new / v_new [B, T, kv heads, hd]");
+  const int64_t T = q.size(1), nh = q.size(2);
+  TORCH_CHECK(q.size(0) == B && q.size(3) == hd && kn.size(0) == B && kn.size(1) == T && kn.size(2) == nkv && kn.size(3) == hd,
+              "q, k_new and v_new must match the caches' batch, kv heads and head dim");
+  TORCH_CHECK(nkv > 0 && nh % nkv == 0, "heads (", str(nh), ") must be a multiple of kv heads (", str(nkv), ")");
+  TORCH_CHECK(q.device() == dev && kn.device() == dev && vn.device() == dev && q.scalar_type() == kc.scalar_type() &&
+                  kn.scalar_type() == kc.scalar_type() && vn.scalar_type() == kc.scalar_type(),
+              "q, k_new and v_new must have the caches' dtype and device");
+  TORCH_CHECK(q.stride(3) == 1 && kn.stride(3) == 1 && vn.stride(3) == 1, "q, k_new, v_new: contiguous head dimension");
+  TORCH_CHECK(hd <= 512, "head dim up to 512, got ", str(hd));
+  TORCH_CHECK(T <= 1024, "at most 1024 new tokens at once, got ", str(T));
+  TORCH_CHECK(B <= 8192, "at most 8192 sequences, got ", str(B));
+  kv_ints(lengths, "lengths", B, dev);
+  KvAttnArgs a{};
+  if (mask && mask->defined()) {
+    TORCH_CHECK(mask->device() == dev && mask->scalar_type() == at::kBool && mask->is_contiguous() &&
+                    mask->size(-1) == T && mask->size(-2) == T &&
+                    (mask->dim() == 2 || (mask->dim() == 3 && (mask->size(0) == B || mask->size(0) == 1))),
+                "mask: contiguous bool [T, T] or [B, T, T]");
+    a.mask = reinterpret_cast<const unsigned char*>(mask->data_ptr<bool>());
+    a.mask_b = mask->dim() == 3 && mask->size(0) == B && B > 1 ? T * T : 0;
+  }
+  if (weight && weight->defined()) {
+    kv_slots(*weight, "weight", at::kFloat, kc);
+    a.weight = weight->data_ptr<float>();
+    a.wt_b = weight->stride(0); a.wt_h = weight->stride(1);
+  }
+  if (positions && positions->defined()) {
+    kv_slots(*positions, "positions", at::kInt, kc);
+    TORCH_CHECK(seen && seen->defined(), "positions need seen");
+    kv_ints(*seen, "seen", B, dev);
+    a.positions = positions->data_ptr<int>();
+    a.pos_b = positions->stride(0); a.pos_h = positions->stride(1);
+    a.seen = seen->data_ptr<int>();
+  }
+  c10::cuda::CUDAGuard guard(dev);
+  at::Tensor o = at::empty({B, T, nh, hd}, q.options());
+  if (o.numel() == 0) return o;
+  a.q = q.data_ptr(); a.kn = kn.data_ptr(); a.vn = vn.data_ptr(); a.kc = kc.data_ptr(); a.vc = vc.data_ptr();
+  a.o = o.data_ptr();
+  a.lengths = lengths.data_ptr<int>();
+  a.q_b = q.stride(0); a.q_t = q.stride(1); a.q_h = q.stride(2);
+  a.kn_b = kn.stride(0); a.kn_t = kn.stride(1); a.kn_h = kn.stride(2);
+  a.vn_b = vn.stride(0); a.vn_t = vn.stride(1); a.vn_h = vn.stride(2);
+  a.kc_b = kc.stride(0); a.kc_h = kc.stride(1); a.kc_s = kc.stride(2);
+  a.vc_b = vc.stride(0); a.vc_h = vc.stride(1); a.vc_s = vc.stride(2);
+  a.B = (int)B; a.T = (int)T; a.nkv = (int)nkv; a.group = (int)(nh / nkv); a.hd = (int)hd; a.S = (int)S;
+  a.scale_log2 = (float)(scale * 1.4426950408889634);
+  kv_attn_plan(a, dt, num_sms(kc));
+  TORCH_CHECK((int64_t)B * nkv * a.nrb < (int64_t)1 << 30, "too many heads and rows");
+  const auto f32 = q.options().dtype(at::kFloat);
+  // one scratch tensor: pieces [2 ctas, rows, hd + 2], then with weights the scores and row sums
+  const int64_t po = 2LL * a.ctas * a.rows * hd, ml = 4LL * a.ctas * a.rows, R = T * (nh / nkv);
+  a.sp = (S + T + 3) / 4 * 4;
+  const int64_t sc = a.weight ? B * nkv * R * a.sp : 0, ls = a.weight ? B * nkv * R : 0;
+  at::Tensor ws = at::empty({po + ml + sc + ls}, f32);
+  a.part_o = ws.data_ptr<float>();
+  a.part_ml = a.part_o + po;
+  if (a.weight) {
+    a.scores = a.part_ml + ml;
+    a.lse = a.scores + sc;
+  }
+  const int rc = kv_attn_launch(a, dt, stream());
+  TORCH_CHECK(rc == 0, "kv_attn launch failed (", str(rc), ")");
+  return o;
+}
+
+std::vector<at::Tensor> kv_evict(at::Tensor kc, at::Tensor vc, at::Tensor weight, at::Tensor positions,
+                                 at::Tensor lengths, at::Tensor seen, int64_t keep, int64_t recent, int64_t sinks,
+                                 c10::optional<at::Tensor> weight_out, c10::optional<at::Tensor> positions_out,
+                                 c10::optional<at::Tensor> lengths_out) {
+  kv_caches(kc, vc, 5);
+  const auto dev = kc.device();
+  const int64_t N = kc.size(0), B = kc.size(1), nkv = kc.size(2), S = kc.size(3), hd = kc.size(4);
+  kv_slots(weight, "weight", at::kFloat, kc);
+  kv_slots(positions, "positions", at::kInt, kc);
+  kv_ints(lengths, "lengths", B, dev);
+  kv_ints(seen, "seen", B, dev);
+  TORCH_CHECK(keep >= 1 && recent >= 0 && sinks >= 0 && recent + sinks <= keep,
+              "keep >= 1 and recent + sinks <= keep, got keep ", str(keep), ", recent ", str(recent), ", sinks ", str(sinks));
+  TORCH_CHECK(N * B * nkv < (int64_t)1 << 26, "too many layers, sequences and heads");
+  c10::cuda::CUDAGuard guard(dev);
+  at::Tensor wo = weight_out && weight_out->defined() ? *weight_out : at::empty(weight.sizes(), weight.options());
+  at::Tensor po = positions_out && positions_out->defined() ? *positions_out : at::empty(positions.sizes(), positions.options());
+  at::Tensor lo = lengths_out && lengths_out->defined() ? *lengths_out : at::empty_like(lengths);
+  kv_slots(wo, "weight output", at::kFloat, kc);
+  kv_slots(po, "positions output", at::kInt, kc);
+  kv_ints(lo, "lengths output", B, dev);
+  TORCH_CHECK((wo.data_ptr() != weight.data_ptr() || wo.strides() == weight.strides()) &&
+                  (po.data_ptr() != positions.data_ptr() || po.strides() == positions.strides()),
+              "an output that is its input must be the whole of it");
+  if (N * B * nkv == 0) return {wo, po, lo};
+  const int64_t cap = std::min(keep, std::max<int64_t>(1, S));
+  at::Tensor ws = at::empty({N * B * nkv * (2 * cap + 1)}, lengths.options());
+  KvEvictArgs a{};
+  a.kc = kc.data_ptr(); a.vc = vc.data_ptr();
+  a.weight = weight.data_ptr<float>(); a.positions = positions.data_ptr<int>();
+  a.lengths = lengths.data_ptr<int>(); a.seen = seen.data_ptr<int>();
+  a.weight_out = wo.data_ptr<float>(); a.positions_out = po.data_ptr<int>(); a.lengths_out = lo.data_ptr<int>();
+  a.kc_n = kc.stride(0); a.kc_b = kc.stride(1); a.kc_h = kc.stride(2); a.kc_s = kc.stride(3);
+  a.vc_n = vc.stride(0); a.vc_b = vc.stride(1); a.vc_h = vc.stride(2); a.vc_s = vc.stride(3);
+  a.w_n = weight.stride(0); a.w_b = weight.stride(1); a.w_h = weight.stride(2);
+  a.p_n = positions.stride(0); a.p_b = positions.stride(1); a.p_h = positions.stride(2);
+  a.wo_n = wo.stride(0); a.wo_b = wo.stride(1); a.wo_h = wo.stride(2);
+  a.po_n = po.stride(0); a.po_b = po.stride(1); a.po_h = po.stride(2);
+  a.N = (int)N; a.B = (int)B; a.nkv = (int)nkv; a.S = (int)S; a.hd = (int)hd; a.esize = (int)kc.element_size();
+  a.keep = (int)cap; a.recent = (int)std::min(recent, cap); a.sinks = (int)std::min(sinks, cap);
+  a.moves = reinterpret_cast<int2*>(ws.data_ptr<int>());
+  a.count = ws.data_ptr<int>() + 2 * N * B * nkv * cap;
+  a.sms = num_sms(kc);
+  const int rc = kv_evict_launch(a, stream());
+  TORCH_CHECK(rc == 0, "kv_evict launch failed (", str(rc), ")");
+  return {wo, po, lo};
+}
+
+std::vector<at::Tensor> kv_commit(at::Tensor parents, at::Tensor tokens, at::Tensor targets, at::Tensor kc, at::Tensor vc,
+                                  at::Tensor lengths, c10::optional<at::Tensor> weight,
+                                  c10::optional<at::Tensor> positions, c10::optional<at::Tensor> seen) {
+  kv_caches(kc, vc, 5);
+  const auto dev = kc.device();
+  const int64_t N = kc.size(0), B = kc.size(1), nkv = kc.size(2), S = kc.size(3), hd = kc.size(4);
+  req(tokens, at::kLong, "tokens");
+  req(targets, at::kLong, "targets");
+  TORCH_CHECK(tokens.dim() == 2 && tokens.size(0) == B && targets.sizes() == tokens.sizes() && tokens.device() == dev &&
+                  targets.device() == dev, "tokens and targets: int64 [B, T] on the caches' device");
+  const int64_t T = tokens.size(1);
+  TORCH_CHECK(T >= 1 && T <= 1024, "a tree has 1 to 1024 nodes, got ", str(T));
+  TORCH_CHECK((parents.dim() == 1 && parents.size(0) == T) || (parents.dim() == 2 && parents.size(0) == B && parents.size(1) == T),
+              "parents: int32 [T] or [B, T]");
+  kv_ints(parents, "parents", parents.numel(), dev);
+  kv_ints(lengths, "lengths", B, dev);
+  KvCommitArgs a{};
+  if (weight && weight->defined()) {
+    kv_slots(*weight, "weight", at::kFloat, kc);
+    a.weight = weight->data_ptr<float>();
+    a.w_n = weight->stride(0); a.w_b = weight->stride(1); a.w_h = weight->stride(2);
+  }
+  if (positions && positions->defined()) {
+    kv_slots(*positions, "positions", at::kInt, kc);
+    TORCH_CHECK(seen && seen->defined(), "positions need seen");
+    kv_ints(*seen, "seen", B, dev);
+    a.positions = positions->data_ptr<int>();
+    a.p_n = positions->stride(0); a.p_b = positions->stride(1); a.p_h = positions->stride(2);
+    a.seen = seen->data_ptr<int>();
+  }
+  c10::cuda::CUDAGuard guard(dev);
+  at::Tensor path = at::empty({B, T}, lengths.options()), count = at::empty({B}, lengths.options());
+  at::Tensor next = at::empty({B}, tokens.options());
+  if (B == 0) return {path, count, next};
+  TORCH_CHECK(N >= 1 && N * B < (int64_t)1 << 30, "at least one layer");
+  a.parents = parents.data_ptr<int>();
+  a.tokens = reinterpret_cast<const long*>(tokens.data_ptr<int64_t>());
+  a.targets = reinterpret_cast<const long*>(targets.data_ptr<int64_t>());
+  a.lengths = lengths.data_ptr<int>();
+  a.kc = kc.data_ptr(); a.vc = vc.data_ptr();
+  a.path = path.data_ptr<int>(); a.count = count.data_ptr<int>();
+  a.next = reinterpret_cast<long*>(next.data_ptr<int64_t>());
+  a.par_b = parents.dim() == 2 ? T : 0;
+  a.kc_n = kc.stride(0); a.kc_b = kc.stride(1); a.kc_h = kc.stride(2); a.kc_s = kc.stride(3);
+  a.vc_n = vc.stride(0); a.vc_b = vc.stride(1); a.vc_h = vc.stride(2); a.vc_s = vc.stride(3);
+  a.N = (int)N; a.B = (int)B; a.T = (int)T; a.nkv = (int)nkv; a.S = (int)S; a.hd = (int)hd;
+  a.esize = (int)kc.element_size();
+  const int rc = kv_commit_launch(a, stream());
+  TORCH_CHECK(rc == 0, "kv_commit launch failed (", str(rc), ")");
+  return {path, count, next};
+}
+
 // ---- attention ----------------------------------------------------------------------------
 static void attn_check(const at::Tensor& t, const char* name, int64_t hd) {
   TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kBFloat16, name, " must be a bf16 CUDA tensor");
@@ -1417,6 +1626,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attn_probsum", &attn_probsum, py::arg("q"), py::arg("k"), py::arg("lse"), py::arg("imp"), py::arg("scale"),
         py::arg("window"), py::arg("q_offset"), py::arg("kpos") = py::none(), py::arg("qoff") = py::none(),
         "head-summed softmax probabilities [B, Lq, Lk] of a finished forward (no gradient)");
+  m.def("kv_attn", &kv_attn, py::arg("q"), py::arg("k_new"), py::arg("v_new"), py::arg("k_cache"), py::arg("v_cache"),
+        py::arg("lengths"), py::arg("mask"), py::arg("scale"), py::arg("weight"), py::arg("positions"), py::arg("seen"),
+        "attention of T new tokens over a key / value cache that stores them (tree mask, accumulated weights)");
+  m.def("kv_evict", &kv_evict, py::arg("k_cache"), py::arg("v_cache"), py::arg("weight"), py::arg("positions"),
+        py::arg("lengths"), py::arg("seen"), py::arg("keep"), py::arg("recent"), py::arg("sinks"),
+        py::arg("weight_out"), py::arg("positions_out"), py::arg("lengths_out"),
+        "eviction from the caches by accumulated weight -> (weight, positions, lengths); rows move in place");
+  m.def("kv_commit", &kv_commit, py::arg("parents"), py::arg("tokens"), py::arg("targets"), py::arg("k_cache"),
+        py::arg("v_cache"), py::arg("lengths"), py::arg("weight"), py::arg("positions"), py::arg("seen"),
+        "acceptance of a drafted tree -> (path, count, next token); the path's rows move behind the cached ones");
   m.def("gdn_scan_fwd", &gdn_scan_fwd,
         "gated delta rule cross-chunk scan: o, the chunk-start states, vnew and the final state");
   m.def("gdn_scan_bwd_value_block", &gdn_scan_bwd_value_block,

@@ -1,0 +1,114 @@
+// Shared parts of the cached-attention kernels (kv_attention.cu, kv_attention_tc.cu): how the
+// keys of all sequences are split over the CTAs, and element types.
+//
+// The lengths live on the device, so the host cannot balance a ragged batch.  Every CTA derives
+// the same split from them instead: the key tiles of all units (sequence, key head, block of query
+// rows) are laid end to end, and CTA c takes tiles [c per, (c + 1) per).  A unit that one CTA holds
+// whole is written out by it; one that several share leaves partial results (unnormalised output,
+// running maximum and sum), which a second kernel joins.  A CTA has at most two such pieces: the
+// end of one unit (slot 2 c) and the beginning of another (slot 2 c + 1).
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <math_constants.h>
+
+#include "common.cuh"
+#include "launchers.h"
+
+namespace s0 {
+namespace kv {
+
+template <typename T> struct Elem;
+template <> struct Elem<float> {
+  S0_DEV static float to(float x) { return x; }
+  S0_DEV static float of(float x) { return x; }
+};
+template <> struct Elem<__half> {
+  S0_DEV static float to(__half x) { return __half2float(x); }
+  S0_DEV static __half of(float x) { return __float2half_rn(x); }
+};
+template <> struct Elem<__nv_bfloat16> {
+  S0_DEV static float to(__nv_bfloat16 x) { return __bfloat162float(x); }
+  S0_DEV static __nv_bfloat16 of(float x) { return __float2bfloat16_rn(x); }
+};
+
+// cached tokens of sequence b: a length outside [0, S] cannot be read or written past the cache
+S0_DEV int cached(const KvAttnArgs& a, int b) { return min(max(__ldg(a.lengths + b), 0), a.S); }
+
+// key tiles of a sequence: its cached tokens, then the new ones (tiles never mix the two)
+S0_DEV int tiles_of(const KvAttnArgs& a, int len, int KT) { return (len + KT - 1) / KT + (a.T + KT - 1) / KT; }
+
+// s_pre[b] = tiles before sequence b of one (head, row block); returns the total.  Called by all
+// threads of the block; needs B + 1 + 32 ints of shared memory.
+S0_DEV long plan_prefix(const KvAttnArgs& a, int KT, int* s_pre) {
+  int* s_w = s_pre + a.B + 1;
+  const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (a.B + nt - 1) / nt, b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
+  int sum = 0;
+  for (int b = b0; b < b1; ++b) sum += tiles_of(a, cached(a, b), KT);
+  int inc = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += y;
+  }
+  if (lane == 31) s_w[warp] = inc;
+  __syncthreads();
+  int base = 0;
+  for (int w = 0; w < warp; ++w) base += s_w[w];
+  int run = base + inc - sum;
+  for (int b = b0; b < b1; ++b) {
+    s_pre[b] = run;
+    run += tiles_of(a, cached(a, b), KT);
+  }
+  if (b1 == a.B && b0 < a.B) s_pre[a.B] = run;
+  __syncthreads();
+  return s_pre[a.B];
+}
+
+struct Plan {
+  long total;  // tiles of all units
+  long per;    // tiles of a CTA
+};
+S0_DEV Plan make_plan(const KvAttnArgs& a, long tiles, int ctas, int min_per) {
+  Plan p;
+  p.total = tiles * a.nkv * a.nrb;
+  p.per = max((long)min_per, (p.total + ctas - 1) / ctas);
+  return p;
+}
+
+// the unit that tile w of the whole line belongs to
+struct Seg {
+  int b, h, rb;  // sequence, key head, row block
+  int len, n;    // cached tokens, tiles of the unit
+  int t0;        // tile w within the unit
+};
+S0_DEV Seg find_seg(const KvAttnArgs& a, const int* s_pre, long w, int KT) {
+  const long hr = (long)a.nkv * a.nrb;
+  int lo = 0, hi = a.B - 1;
+  while (lo < hi) {  // the last b with pre[b] * hr <= w
+    const int mid = (lo + hi + 1) >> 1;
+    if ((long)s_pre[mid] * hr <= w) lo = mid; else hi = mid - 1;
+  }
+  Seg s;
+  s.b = lo;
+  s.len = cached(a, lo);
+  s.n = s_pre[lo + 1] - s_pre[lo];
+  const long rem = w - (long)s_pre[lo] * hr;
+  const int u = (int)(rem / s.n);
+  s.t0 = (int)(rem - (long)u * s.n);
+  s.h = u / a.nrb;
+  s.rb = u - s.h * a.nrb;
+  return s;
+}
+
+// the mask row of new token t: which new tokens it sees
+S0_DEV bool sees(const KvAttnArgs& a, int b, int t, int i) {
+  return a.mask ? a.mask[b * a.mask_b + (long)t * a.T + i] != 0 : i <= t;
+}
+
+// base-2 log-sum-exp of a row; +inf where it saw nothing, so that exp2(s - lse) is 0 there
+S0_DEV float lse2(float m, float l) { return l == 0.f ? CUDART_INF_F : m + log2f(l); }
+
+}  // namespace kv
+}  // namespace s0

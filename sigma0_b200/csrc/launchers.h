@@ -355,3 +355,62 @@ struct GdnDecodeArgs {
   int B, T, nh, hvd, alog_dim;
 };
 int gdn_decode_launch(const GdnDecodeArgs& a, int hd, cudaStream_t st);
+
+// attention of T new tokens over a key / value cache (kv_attention.cu); strides in elements, the
+// head dimension contiguous.  dtype: 0 float, 1 half, 2 bfloat16
+struct KvAttnArgs {
+  const void *q, *kn, *vn;            // [B, T, nkv * group, hd], [B, T, nkv, hd] (strided)
+  void *kc, *vc;                      // [B, nkv, S, hd] (strided): rows [len, len + T) are written
+  void* o;                            // [B, T, nkv * group, hd] contiguous
+  const int* lengths;                 // [B] cached tokens
+  const unsigned char* mask;          // [B, T, T] which new tokens a row sees (nullptr: causal)
+  float* weight;                      // optional [B, nkv, S]: the rows' probabilities are added
+  int* positions;                     // optional [B, nkv, S]: new rows get seen[b] + their index
+  const int* seen;                    // [B]
+  long q_b, q_t, q_h, kn_b, kn_t, kn_h, vn_b, vn_t, vn_h, kc_b, kc_h, kc_s, vc_b, vc_h, vc_s;
+  long mask_b, wt_b, wt_h, pos_b, pos_h;  // mask_b 0: one mask for all sequences
+  int B, T, nkv, group, hd, S;
+  float scale_log2;                   // softmax scale * log2(e)
+  // set by kv_attn_plan: rows of a block, row blocks, CTAs, least tiles of a CTA
+  int rows, nrb, ctas, min_per;
+  // scratch: 2 * ctas pieces of [rows, hd] and [rows, 2]; with weights [B, nkv, T * group, sp] scores
+  // and [B, nkv, T * group] log-sum-exps
+  float *part_o, *part_ml, *scores, *lse;
+  long sp;
+};
+void kv_attn_plan(KvAttnArgs& a, int dtype, int sms);
+int kv_attn_launch(const KvAttnArgs& a, int dtype, cudaStream_t st);
+
+// eviction from caches by accumulated weight (kv_evict.cu): N layers, B sequences, nkv heads
+struct KvEvictArgs {
+  void *kc, *vc;                      // [N, B, nkv, S, hd] (strided), rows move in place
+  const float* weight;                // [N, B, nkv, S] (strided, slots contiguous)
+  const int* positions;               // the same
+  const int *lengths, *seen;          // [B]
+  float* weight_out;                  // may be weight
+  int* positions_out;                 // may be positions
+  int* lengths_out;                   // may be lengths
+  long kc_n, kc_b, kc_h, kc_s, vc_n, vc_b, vc_h, vc_s;
+  long w_n, w_b, w_h, p_n, p_b, p_h, wo_n, wo_b, wo_h, po_n, po_b, po_h;
+  int N, B, nkv, S, hd, esize;
+  int keep, recent, sinks;
+  int2* moves;                        // scratch [N * B * nkv, keep]: (from, to) slots
+  int* count;                         // scratch [N * B * nkv]
+  int sms;
+};
+int kv_evict_launch(const KvEvictArgs& a, cudaStream_t st);
+
+// acceptance of a drafted tree (kv_evict.cu)
+struct KvCommitArgs {
+  const int* parents;                 // [B, T], -1 at the root (par_b 0: one tree for all sequences)
+  const long *tokens, *targets;       // [B, T] drafted tokens, the model's token after each node
+  const int *lengths, *seen;          // [B]
+  void *kc, *vc;                      // [N, B, nkv, S, hd] (strided)
+  float* weight;                      // optional [N, B, nkv, S]
+  int* positions;                     // optional [N, B, nkv, S]
+  int *path, *count;                  // [B, T] (-1 behind the path), [B]
+  long* next;                         // [B]
+  long par_b, kc_n, kc_b, kc_h, kc_s, vc_n, vc_b, vc_h, vc_s, w_n, w_b, w_h, p_n, p_b, p_h;
+  int N, B, T, nkv, S, hd, esize;
+};
+int kv_commit_launch(const KvCommitArgs& a, cudaStream_t st);

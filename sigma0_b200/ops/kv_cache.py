@@ -1,0 +1,206 @@
+"""Decoding over a key / value cache: attention of new tokens, eviction, acceptance of drafts.
+
+A cache is a pair of tensors ``[B, kv_heads, slots, head_dim]`` (one layer; the eviction and the
+acceptance also take ``[layers, B, kv_heads, slots, head_dim]``) of which the first ``lengths[b]``
+slots of sequence ``b`` hold tokens.  Lengths are int32 on the device and nothing here reads them
+on the host, so sequences of different lengths share a batch and a step can be captured in a CUDA
+graph.  The order of the cached rows means nothing to the attention; ``positions`` (int32, the
+cache's shape without the head dimension, -1 in free slots) says which token a slot holds and
+``weight`` (float32, 0 in free slots) how much softmax weight it has received.
+
+* :func:`cache_attention` stores the keys and values of T new tokens in slots ``[len, len + T)``
+  and attends from them; ``lengths`` stays as it is until the caller adds the tokens that it keeps.
+* :func:`cache_evict` cuts every layer and head to ``keep`` tokens by accumulated weight.
+* :func:`tree_commit` accepts the longest path of a drafted tree that agrees with the model.
+
+CUDA tensors run the kernels of ``csrc/kv_attention.cu``, ``csrc/kv_attention_tc.cu`` and
+``csrc/kv_evict.cu``; CPU tensors the torch expressions below.  Inference only: none of them has
+a gradient.  The reference decodes one token at a time over a static cache that only grows
+(``src/base_model/models/transformer.py:285-392``).
+"""
+from __future__ import annotations
+
+import torch
+
+from ._ext import ext
+
+
+def tree_mask(parents: torch.Tensor) -> torch.Tensor:
+    """bool [..., T, T] of int parents [..., T] (-1: no parent): row i sees its ancestors and itself.
+
+    A parent has a lower index than its children."""
+    T = parents.shape[-1]
+    m = torch.eye(T, dtype=torch.bool, device=parents.device).expand(*parents.shape, T).clone()
+    for i in range(1, T):
+        p = parents[..., i].long()
+        up = m.gather(-2, p.clamp_min(0)[..., None, None].expand(*p.shape, 1, T))[..., 0, :]
+        m[..., i, :] |= up & (p >= 0)[..., None]
+    return m
+
+
+def tree_depth(mask: torch.Tensor) -> torch.Tensor:
+    """int64 [..., T] depth of every node (0 at the root) from its ancestor mask."""
+    return mask.sum(-1) - 1
+
+
+def _inference_only(*ts):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+        raise RuntimeError("decoding over a cache has no gradient: call it under torch.no_grad()")
+
+
+def cache_attention(q, k_new, v_new, k_cache, v_cache, lengths, mask=None, scale=None, weight=None, positions=None,
+                    seen=None):
+    """Attention of T new tokens over the cached tokens and one another -> [B, T, heads, hd].
+
+    q [B, T, heads, hd], k_new / v_new [B, T, kv_heads, hd], caches [B, kv_heads, slots, hd], all of one
+    dtype (float32, float16, bfloat16; hd <= 512, T <= 1024) and ``heads`` a multiple of ``kv_heads``.
+    Every new token sees the ``lengths[b]`` cached ones and those new ones that its row of ``mask``
+    (bool [T, T] or [B, T, T]; None: causal) names; a row that sees nothing gives zeros, and a NaN or an
+    infinity in a token shows in no row that does not see it.  The new rows are stored in slots ``lengths[b] ...``; rows past the last slot are attended to but not stored.
+
+    ``weight`` [B, kv_heads, slots] gets the probabilities of all T rows and of the group's query heads
+    added, ``positions`` the value ``seen[b] + i`` for new token i (both in place)."""
+    _inference_only(q, k_new, v_new, k_cache, v_cache)
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    if k_cache.is_cuda:
+        return ext().kv_attn(q, k_new, v_new, k_cache, v_cache, lengths, mask, scale, weight, positions, seen)
+    return _attention_torch(q, k_new, v_new, k_cache, v_cache, lengths, mask, scale, weight, positions, seen)
+
+
+def cache_evict(k_cache, v_cache, weight, positions, lengths, seen, keep, recent=0, sinks=0, out=None):
+    """Cut every sequence, layer and head to ``keep`` tokens -> (weight, positions, lengths).
+
+    The tokens at positions below ``sinks`` and the ``recent`` last ones (positions from
+    ``seen[b] - recent``; ``seen[b]`` tokens have been through the sequence) stay, then those with the most
+    ``weight`` (the lower slot among equals; NaN counts as the most).  Rows of survivors behind the new
+    end move into free slots before it, in place.  A sequence of at most ``keep`` tokens stays as it is.
+    Slots from the new length on get weight 0 and position -1.  ``out``: three tensors for the results,
+    which may be the inputs themselves."""
+    kc, vc, w, p = (x if x.dim() > n else x.unsqueeze(0) for x, n in
+                    ((k_cache, 4), (v_cache, 4), (weight, 3), (positions, 3)))
+    ow, op, ol = out if out is not None else (None, None, None)
+    if out is not None and ow.dim() == 3:
+        ow, op = ow.unsqueeze(0), op.unsqueeze(0)
+    if k_cache.is_cuda:
+        ow, op, ol = ext().kv_evict(kc, vc, w, p, lengths, seen, int(keep), int(recent), int(sinks), ow, op, ol)
+    else:
+        res = _evict_torch(kc, vc, w, p, lengths, seen, int(keep), int(recent), int(sinks))
+        if out is not None:
+            for o, r in zip((ow, op, ol), res):
+                o.copy_(r)
+        else:
+            ow, op, ol = res
+    if out is not None:
+        return tuple(out)
+    return (ow, op, ol) if weight.dim() == 4 else (ow[0], op[0], ol)
+
+
+def tree_commit(parents, tokens, targets, k_cache, v_cache, lengths, weight=None, positions=None, seen=None):
+    """Accept the longest root path of a drafted tree that the model agrees with -> (path, count, token).
+
+    Node 0 of the T nodes is the last accepted token; node i hangs below node ``parents[i] < i`` (int32 [T]
+    or [B, T]), drafts ``tokens[b, i]`` (int64) and the model continues it with ``targets[b, i]``.  From the
+    root the walk goes to the lowest child whose token is the model's, until there is none: ``path``
+    int32 [B, T] holds its nodes (-1 behind them), ``count`` int32 [B] how many, ``token`` int64 [B] the
+    model's token after the last.  The path's rows, which :func:`cache_attention` left in slots
+    ``lengths[b] + node``, move up to ``lengths[b] + 0, 1, ...`` in all layers; ``weight`` follows and is 0
+    for the dropped ones, ``positions`` become ``seen[b] + 0, 1, ...`` and -1.  ``lengths`` and ``seen``
+    stay as they are: add ``count`` to them."""
+    kc, vc = (x if x.dim() > 4 else x.unsqueeze(0) for x in (k_cache, v_cache))
+    w, p = (x if x is None or x.dim() > 3 else x.unsqueeze(0) for x in (weight, positions))
+    if k_cache.is_cuda:
+        return tuple(ext().kv_commit(parents, tokens, targets, kc, vc, lengths, w, p, seen))
+    return _commit_torch(parents, tokens, targets, kc, vc, lengths, w, p, seen)
+
+
+# ---- torch expressions (CPU tensors) ------------------------------------------------------------
+def _attention_torch(q, k_new, v_new, kc, vc, lengths, mask, scale, weight, positions, seen):
+    B, T, nh, hd = q.shape
+    nkv, S = kc.shape[1], kc.shape[2]
+    if nh % nkv or k_new.shape != (B, T, nkv, hd) or v_new.shape != k_new.shape or kc.shape != vc.shape:
+        raise ValueError("q, k_new and v_new must match the caches' batch, kv heads and head dim")
+    if positions is not None and seen is None:
+        raise ValueError("positions need seen")
+    new = torch.ones(T, T, dtype=torch.bool).tril() if mask is None else mask
+    new = new.expand(B, T, T)
+    o = torch.zeros(B, T, nh, hd, dtype=q.dtype)
+    for b in range(B):
+        n = min(max(int(lengths[b]), 0), S)
+        k = torch.cat([kc[b, :, :n], k_new[b].transpose(0, 1)], 1).float()
+        v = torch.cat([vc[b, :, :n], v_new[b].transpose(0, 1)], 1).float()
+        qf = q[b].float().reshape(T, nkv, nh // nkv, hd).permute(1, 2, 0, 3)
+        s = qf @ k[:, None].transpose(-1, -2) * scale
+        hide = torch.cat([torch.zeros(T, n, dtype=torch.bool), ~new[b]], 1)
+        p = torch.softmax(s.masked_fill(hide, float("-inf")), -1).masked_fill(hide.all(-1, keepdim=True), 0.0)
+        if torch.isfinite(v_new[b]).all():
+            x = p @ v[:, None]
+        else:                                    # 0 times an infinity: what a row does not see adds nothing
+            x = (p[..., None] * v[:, None, None]).masked_fill(hide[..., None], 0.0).sum(-2)
+        o[b] = x.permute(2, 0, 1, 3).reshape(T, nh, hd).to(q.dtype)
+        fit = min(T, S - n)
+        if weight is not None:
+            weight[b, :, :n + fit] += p.sum((1, 2))[:, :n + fit]
+        kc[b, :, n:n + fit] = k_new[b, :fit].transpose(0, 1)
+        vc[b, :, n:n + fit] = v_new[b, :fit].transpose(0, 1)
+        if positions is not None:
+            positions[b, :, n:n + fit] = seen[b] + torch.arange(fit, dtype=torch.int32)
+    return o
+
+
+def _evict_torch(kc, vc, w, pos, lengths, seen, keep, recent, sinks):
+    if keep < 1 or recent < 0 or sinks < 0 or recent + sinks > keep:
+        raise ValueError("keep >= 1 and recent + sinks <= keep")
+    S = w.shape[-1]
+    slot = torch.arange(S)
+    ls = lengths.long().clamp(0, S)[:, None, None]
+    new = ls.clamp_max(keep)
+    # float64 leaves room above every float32 weight for NaN and the held positions
+    key = w.double().clamp(-1e300, 1e300)
+    key = key.masked_fill(w.isnan(), 1e301)
+    key = key.masked_fill((pos >= seen[:, None, None] - recent) | (pos < sinks), 1e302)
+    order = key.masked_fill(slot >= ls, float("-inf")).sort(dim=-1, descending=True, stable=True).indices
+    stays = torch.empty_like(order).scatter_(-1, order, slot.expand_as(order)) < new
+    hole, mover = (slot < new) & ~stays, (slot >= new) & stays
+    frm = torch.where(mover, slot, S).sort(-1).values
+    src = torch.where(hole, frm.gather(-1, (hole.cumsum(-1) - 1).clamp_min(0)), slot).clamp_max(max(S - 1, 0))
+    rows = src[..., None].expand(kc.shape)
+    kc.copy_(torch.where(hole[..., None], kc.gather(-2, rows), kc))
+    vc.copy_(torch.where(hole[..., None], vc.gather(-2, rows), vc))
+    gone = slot >= new
+    return (w.gather(-1, src).masked_fill(gone, 0.0), pos.gather(-1, src).masked_fill(gone, -1),
+            lengths.clamp(0, S).clamp_max(keep))
+
+
+def _commit_torch(parents, tokens, targets, kc, vc, lengths, weight, positions, seen):
+    if positions is not None and seen is None:
+        raise ValueError("positions need seen")
+    B, T = tokens.shape
+    S = kc.shape[3]
+    par = parents.expand(B, T).tolist()
+    path = torch.full((B, T), -1, dtype=torch.int32)
+    count = torch.empty(B, dtype=torch.int32)
+    token = torch.empty(B, dtype=torch.int64)
+    for b in range(B):
+        walk = [0]
+        while True:
+            cur = walk[-1]
+            nxt = next((i for i in range(cur + 1, T) if par[b][i] == cur and tokens[b, i] == targets[b, cur]), None)
+            if nxt is None:
+                break
+            walk.append(nxt)
+        n = min(max(int(lengths[b]), 0), S)
+        fit = min(T, S - n)
+        keep = [i for i in walk if i < fit]
+        rows = torch.tensor([n + i for i in keep], dtype=torch.long)
+        for cache in (kc, vc):
+            cache[:, b, :, n:n + len(keep)] = cache[:, b].index_select(2, rows)
+        if weight is not None:
+            was = weight[:, b].index_select(2, rows)
+            weight[:, b, :, n:n + fit] = 0.0
+            weight[:, b, :, n:n + len(keep)] = was
+        if positions is not None:
+            positions[:, b, :, n:n + fit] = -1
+            positions[:, b, :, n:n + len(keep)] = seen[b] + torch.arange(len(keep), dtype=torch.int32)
+        path[b, :len(walk)] = torch.tensor(walk, dtype=torch.int32)
+        count[b], token[b] = len(walk), targets[b, walk[-1]]
+    return path, count, token
