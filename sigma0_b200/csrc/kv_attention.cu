@@ -257,14 +257,17 @@ __global__ void __launch_bounds__(JT) kv_join_k(KvAttnArgs a, int KT, int ctas) 
 template <typename T>
 int launch(const KvAttnArgs& a, cudaStream_t st) {
   const size_t sm = (size_t)(GR * a.hd + GK * (a.hd | 1) + GR * GK + 2 * GR) * 4 + (size_t)(a.B + 33) * 4;
-  cudaError_t e = cudaFuncSetAttribute(kv_attn_any_k<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
+  const cudaError_t e = cudaFuncSetAttribute(kv_attn_any_k<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
   if (e != cudaSuccess) return (int)e;
   kv_attn_any_k<T><<<a.ctas, GT, sm, st>>>(a);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return (int)e;
+  return (int)cudaGetLastError();
+}
+
+template <typename T>
+int join(const KvAttnArgs& a, cudaStream_t st) {
   const long units = (long)a.B * a.nkv * a.nrb;
   const long wblocks = a.weight ? (long)a.B * a.nkv * ((a.S + a.T + JW - 1) / JW) : 0;
-  kv_join_k<T><<<(unsigned)(units + wblocks), JT, (size_t)(a.B + 33) * 4, st>>>(a, GK, a.ctas);
+  kv_join_k<T><<<(unsigned)(units + wblocks), JT, (size_t)(a.B + 33) * 4, st>>>(a, a.tile, a.ctas);
   return (int)cudaGetLastError();
 }
 
@@ -272,17 +275,23 @@ int launch(const KvAttnArgs& a, cudaStream_t st) {
 }  // namespace s0
 
 void kv_attn_plan(KvAttnArgs& a, int dtype, int sms) {
+  a.tc = kv_attn_tc_takes(a, dtype);
+  if (a.tc) return kv_attn_tc_plan(a, sms);
   const size_t sm = (size_t)(s0::kv::GR * a.hd + s0::kv::GK * (a.hd | 1) + s0::kv::GR * s0::kv::GK) * 4;
   const int R = a.T * a.group;
   a.rows = s0::kv::GR;
   a.nrb = (R + a.rows - 1) / a.rows;
+  a.tile = s0::kv::GK;
   a.min_per = 4;
+  a.whole = 0;
   a.ctas = sms * (int)std::max<size_t>(1, std::min<size_t>(8, (size_t)200 * 1024 / sm));
 }
 
 int kv_attn_launch(const KvAttnArgs& a, int dtype, cudaStream_t st) {
   if (a.B <= 0 || a.T <= 0) return 0;
-  if (dtype == 0) return s0::kv::launch<float>(a, st);
-  if (dtype == 1) return s0::kv::launch<__half>(a, st);
-  return s0::kv::launch<__nv_bfloat16>(a, st);
+  using namespace s0::kv;
+  const int rc = a.tc ? kv_attn_tc_launch(a, dtype, st)
+                 : dtype == 0 ? launch<float>(a, st) : dtype == 1 ? launch<__half>(a, st) : launch<__nv_bfloat16>(a, st);
+  if (rc) return rc;
+  return dtype == 0 ? join<float>(a, st) : dtype == 1 ? join<__half>(a, st) : join<__nv_bfloat16>(a, st);
 }

@@ -371,13 +371,17 @@ struct KvAttnArgs {
   long mask_b, wt_b, wt_h, pos_b, pos_h;  // mask_b 0: one mask for all sequences
   int B, T, nkv, group, hd, S;
   float scale_log2;                   // softmax scale * log2(e)
-  // set by kv_attn_plan: rows of a block, row blocks, CTAs, least tiles of a CTA
-  int rows, nrb, ctas, min_per;
+  // set by kv_attn_plan: rows of a block, row blocks, keys of a tile, CTAs, least tiles of a CTA, one
+  // CTA per unit (no split), tensor cores
+  int rows, nrb, tile, ctas, min_per, whole, tc;
   // scratch: 2 * ctas pieces of [rows, hd] and [rows, 2]; with weights [B, nkv, T * group, sp] scores
   // and [B, nkv, T * group] log-sum-exps
   float *part_o, *part_ml, *scores, *lse;
   long sp;
 };
+bool kv_attn_tc_takes(const KvAttnArgs& a, int dtype);
+void kv_attn_tc_plan(KvAttnArgs& a, int sms);
+int kv_attn_tc_launch(const KvAttnArgs& a, int dtype, cudaStream_t st);
 void kv_attn_plan(KvAttnArgs& a, int dtype, int sms);
 int kv_attn_launch(const KvAttnArgs& a, int dtype, cudaStream_t st);
 
