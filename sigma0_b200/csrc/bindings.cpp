@@ -809,6 +809,8 @@ at::Tensor kv_attn(at::Tensor q, at::Tensor kn, at::Tensor vn, at::Tensor kc, at
               "q, k_new and v_new must have the caches' dtype and device");
   TORCH_CHECK(q.stride(3) == 1 && kn.stride(3) == 1 && vn.stride(3) == 1, "q, k_new, v_new: contiguous head dimension");
   TORCH_CHECK(hd <= 512, "head dim up to 512, got ", str(hd));
+  TORCH_CHECK(scale > 0 && scale < 1e30, "scale must be positive");
+  TORCH_CHECK(nh / nkv <= 1024, "at most 1024 heads over one kv head");
   TORCH_CHECK(T <= 1024, "at most 1024 new tokens at once, got ", str(T));
   TORCH_CHECK(B <= 8192, "at most 8192 sequences, got ", str(B));
   kv_ints(lengths, "lengths", B, dev);
@@ -847,20 +849,22 @@ at::Tensor kv_attn(at::Tensor q, at::Tensor kn, at::Tensor vn, at::Tensor kc, at
   a.vc_b = vc.stride(0); a.vc_h = vc.stride(1); a.vc_s = vc.stride(2);
   a.B = (int)B; a.T = (int)T; a.nkv = (int)nkv; a.group = (int)(nh / nkv); a.hd = (int)hd; a.S = (int)S;
   a.scale_log2 = (float)(scale * 1.4426950408889634);
+  a.inv_group = 1.f / (float)a.group;
   kv_attn_plan(a, dt, num_sms(kc));
-  TORCH_CHECK((int64_t)B * nkv * a.nrb < (int64_t)1 << 30, "too many heads and rows");
+  TORCH_CHECK(B * nh * T < (int64_t)1 << 30 && B * nkv * ((S + T) / 2048 + 1) < (int64_t)1 << 30, "too many heads and rows");
   const auto f32 = q.options().dtype(at::kFloat);
   // one scratch tensor: pieces [2 ctas, rows, hd + 2], then with weights the scores and row sums
   const int64_t po = 2LL * a.ctas * a.rows * hd, ml = 4LL * a.ctas * a.rows, R = T * (nh / nkv);
   a.sp = (S + T + 3) / 4 * 4;
   const int64_t sc = a.weight ? B * nkv * R * a.sp : 0, ls = a.weight ? B * nkv * R : 0;
-  at::Tensor ws = at::empty({po + ml + sc + ls}, f32);
+  at::Tensor ws = at::empty({po + ml + sc + ls + B + 1}, f32);
   a.part_o = ws.data_ptr<float>();
   a.part_ml = a.part_o + po;
   if (a.weight) {
     a.scores = a.part_ml + ml;
     a.lse = a.scores + sc;
   }
+  a.prefix = reinterpret_cast<int*>(a.part_ml + ml + sc + ls);
   const int rc = kv_attn_launch(a, dt, stream());
   TORCH_CHECK(rc == 0, "kv_attn launch failed (", str(rc), ")");
   return o;

@@ -35,7 +35,10 @@ __global__ void __launch_bounds__(GT) kv_attn_any_k(KvAttnArgs a) {
   int* s_pre = reinterpret_cast<int*>(sV + GR);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int R = a.T * a.group;
+  join_may_start();
   const Plan plan = make_plan(a, plan_prefix(a, GK, s_pre), gridDim.x, a.min_per);
+  if (blockIdx.x == 0)
+    for (int i = tid; i <= a.B; i += GT) a.prefix[i] = s_pre[i];
   long w = blockIdx.x * plan.per;
   const long wend = min(plan.total, w + plan.per);
 
@@ -174,78 +177,119 @@ __global__ void __launch_bounds__(GT) kv_attn_any_k(KvAttnArgs a) {
 }
 
 // Joins the pieces of the units that several CTAs share, and adds up the weights.  Blocks
-// [0, units): the output of one unit; the others: 1024 slots of one (sequence, key head) each.
-constexpr int JT = 256, JW = 1024;
+// [0, B heads T): one row's output; the others: JW slots of one (sequence, key head) each.
+constexpr int JT = 256, JW = 2048;
 
-template <typename T>
-__global__ void __launch_bounds__(JT) kv_join_k(KvAttnArgs a, int KT, int ctas) {
-  extern __shared__ __align__(16) unsigned char smem[];
-  int* s_pre = reinterpret_cast<int*>(smem);
-  __shared__ float s_lse[JT];
-  const int tid = threadIdx.x, R = a.T * a.group;
-  const Plan plan = make_plan(a, plan_prefix(a, KT, s_pre), ctas, a.min_per);
-  const long units = (long)a.B * a.nkv * a.nrb;
-  const bool out = blockIdx.x < units;
-  const long wb = blockIdx.x - units;
-  const int nch = (a.S + a.T + JW - 1) / JW;
-  const long bh = out ? (long)blockIdx.x / a.nrb : wb / nch;
-  const int b = (int)(bh / a.nkv), h = (int)(bh % a.nkv);
-  const int n = s_pre[b + 1] - s_pre[b];
-  const long ub = (long)s_pre[b] * a.nkv * a.nrb + (long)h * a.nrb * n;   // first tile of row block 0
-  // piece i of row block rb: CTA c0 + i
-  auto slot_of = [](long c, long c0) { return 2 * c + (c == c0 ? 1 : 0); };
+struct Pieces {
+  long c0, c1;  // first and last CTA of the unit
+};
+// piece of CTA c: see kv_attention.cuh
+S0_DEV long piece(const KvAttnArgs& a, const Pieces& p, long c, int r) { return (2 * c + (c == p.c0 ? 1 : 0)) * a.rows + r; }
+// one warp: maximum and sum of a row over its pieces
+S0_DEV void row_sum(const KvAttnArgs& a, const Pieces& p, int r, float& M, float& L) {
+  const int lane = threadIdx.x & 31;
+  M = -CUDART_INF_F;
+  L = 0.f;
+  for (long c = p.c0 + lane; c <= p.c1; c += 32) M = fmaxf(M, a.part_ml[piece(a, p, c, r) * 2]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  const float base = M == -CUDART_INF_F ? 0.f : M;
+  for (long c = p.c0 + lane; c <= p.c1; c += 32) {
+    const long i = piece(a, p, c, r) * 2;
+    L += a.part_ml[i + 1] * ex2(a.part_ml[i] - base);
+  }
+  L = warp_sum(L);
+}
 
+// WPR warps share the pieces of a row
+template <typename T, int WPR>
+__global__ void __launch_bounds__(JT) kv_join_k(KvAttnArgs a, int row_blocks) {
+  constexpr int RPB = JT / 32 / WPR, COLS = 4;     // rows of a block, columns of a lane at a time
+  __shared__ float s_x[JT * COLS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, R = a.T * a.group;
+  const bool out = blockIdx.x < (unsigned)row_blocks;
+  const int wb = blockIdx.x - row_blocks, nch = (a.S + a.T + JW - 1) / JW;
+  const long total = (long)a.B * a.nkv * R, idx = (long)blockIdx.x * RPB + warp / WPR;
+  const long bh = out ? min(idx, total - 1) / R : wb / nch;
+  const int b = (int)(bh / a.nkv), h = (int)(bh - (long)b * a.nkv);
+  join_wait();
+  Plan plan{0, 1};
+  int n = 1;
+  long ub = 0;                                      // first tile of row block 0
+  if (!a.whole) {
+    plan = make_plan(a, a.prefix[a.B], a.ctas, a.min_per);
+    const int p0 = a.prefix[b];
+    n = a.prefix[b + 1] - p0;
+    ub = (long)p0 * a.nkv * a.nrb + (long)h * a.nrb * n;
+  }
+  auto pieces = [&](int rb) {
+    const long s = ub + (long)rb * n;
+    return Pieces{s / plan.per, (s + n - 1) / plan.per};
+  };
   if (out) {
-    const int rb = (int)(blockIdx.x % a.nrb), r0 = rb * a.rows, nr = min(a.rows, R - r0);
-    const long s = ub + (long)rb * n, c0 = s / plan.per, c1 = (s + n - 1) / plan.per;
-    if (c0 == c1) return;
-    for (int i = tid; i < nr * a.hd; i += JT) {
-      const int r = i / a.hd, d = i - r * a.hd;
-      float M = -CUDART_INF_F, L = 0.f, x = 0.f;
-      for (long c = c0; c <= c1; ++c) {
-        const long slot = slot_of(c, c0) * a.rows + r;
-        const float mi = a.part_ml[slot * 2], li = a.part_ml[slot * 2 + 1], mn = fmaxf(M, mi);
-        const float base = mn == -CUDART_INF_F ? 0.f : mn, e0 = exp2f(M - base), e1 = exp2f(mi - base);
-        L = L * e0 + li * e1;
-        x = x * e0 + a.part_o[slot * a.hd + d] * e1;
-        M = mn;
+    const int row = (int)(min(idx, total - 1) - bh * R), rb = row / a.rows, r = row - rb * a.rows;
+    const Pieces p = pieces(rb);
+    if ((WPR > 1 || idx < total) && p.c0 == p.c1) return;      // WPR > 1: one row in the block, all leave
+    if (WPR == 1 && idx >= total) return;
+    float M, L;
+    row_sum(a, p, r, M, L);
+    const float base = M == -CUDART_INF_F ? 0.f : M, inv = L == 0.f ? 0.f : 1.f / L;
+    const int t = row / a.group, g = row - t * a.group;
+    T* o = (T*)a.o + (((long)b * a.T + t) * a.nkv * a.group + h * a.group + g) * a.hd;
+    for (int d0 = lane; d0 - lane < a.hd; d0 += 32 * COLS) {
+      float x[COLS] = {};
+#pragma unroll 4
+      for (long c = p.c0 + warp % WPR; c <= p.c1; c += WPR) {
+        const long i = piece(a, p, c, r);
+        const float f = ex2(a.part_ml[i * 2] - base);
+#pragma unroll
+        for (int k = 0; k < COLS; ++k)
+          if (d0 + 32 * k < a.hd) x[k] = fmaf(a.part_o[i * a.hd + d0 + 32 * k], f, x[k]);
       }
-      const int row = r0 + r, t = row / a.group, g = row - t * a.group;
-      ((T*)a.o)[(((long)b * a.T + t) * a.nkv * a.group + h * a.group + g) * a.hd + d] =
-          Elem<T>::of(L == 0.f ? 0.f : x / L);
+      if constexpr (WPR > 1) {
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < COLS; ++k) s_x[(warp * COLS + k) * 32 + lane] = x[k];
+        __syncthreads();
+        if (warp == 0) {
+#pragma unroll
+          for (int k = 0; k < COLS; ++k)
+            for (int w = 1; w < WPR; ++w) x[k] += s_x[(w * COLS + k) * 32 + lane];
+        }
+      }
+      if (WPR == 1 || warp == 0) {
+#pragma unroll
+        for (int k = 0; k < COLS; ++k)
+          if (d0 + 32 * k < a.hd) o[d0 + 32 * k] = Elem<T>::of(x[k] * inv);
+      }
     }
     return;
   }
-  const int len = cached(a, b), hi = min(a.S, len + a.T), j0 = (int)(wb % nch) * JW;
+  const int hi = min(a.S, cached(a, b) + a.T), j0 = (wb - (int)bh * nch) * JW;
   if (j0 >= hi) return;
   float add[JW / JT] = {};
   for (int q0 = 0; q0 < R; q0 += JT) {
-    const int row = q0 + tid;
     __syncthreads();
-    if (row < R) {
-      const int rb = row / a.rows, r = row - rb * a.rows;
-      const long s = ub + (long)rb * n, c0 = s / plan.per, c1 = (s + n - 1) / plan.per;
-      if (c0 == c1) {
-        s_lse[tid] = a.lse[bh * R + row];
+    for (int q = warp; q < min(JT, R - q0); q += JT / 32) {
+      const int row = q0 + q, rb = row / a.rows;
+      const Pieces p = pieces(rb);
+      float x;
+      if (p.c0 == p.c1) {
+        x = a.lse[bh * R + row];
       } else {
-        float M = -CUDART_INF_F, L = 0.f;
-        for (long c = c0; c <= c1; ++c) {
-          const long slot = slot_of(c, c0) * a.rows + r;
-          const float mi = a.part_ml[slot * 2], li = a.part_ml[slot * 2 + 1], mn = fmaxf(M, mi);
-          const float base = mn == -CUDART_INF_F ? 0.f : mn;
-          L = L * exp2f(M - base) + li * exp2f(mi - base);
-          M = mn;
-        }
-        s_lse[tid] = lse2(M, L);
+        float M, L;
+        row_sum(a, p, row - rb * a.rows, M, L);
+        x = lse2(M, L);
       }
+      if (lane == 0) s_x[q] = x;
     }
     __syncthreads();
     for (int q = 0; q < min(JT, R - q0); ++q) {
       const float* sc = a.scores + (bh * R + q0 + q) * a.sp + j0;
-      const float ls = s_lse[q];
+      const float ls = s_x[q];
 #pragma unroll
       for (int i = 0; i < JW / JT; ++i)
-        if (j0 + i * JT + tid < hi) add[i] += exp2f(sc[i * JT + tid] - ls);
+        if (j0 + i * JT + tid < hi) add[i] += ex2(sc[i * JT + tid] - ls);
     }
   }
   float* wt = a.weight + b * a.wt_b + h * a.wt_h + j0;
@@ -265,10 +309,23 @@ int launch(const KvAttnArgs& a, cudaStream_t st) {
 
 template <typename T>
 int join(const KvAttnArgs& a, cudaStream_t st) {
-  const long units = (long)a.B * a.nkv * a.nrb;
-  const long wblocks = a.weight ? (long)a.B * a.nkv * ((a.S + a.T + JW - 1) / JW) : 0;
-  kv_join_k<T><<<(unsigned)(units + wblocks), JT, (size_t)(a.B + 33) * 4, st>>>(a, a.tile, a.ctas);
-  return (int)cudaGetLastError();
+  // few rows leave room for a block each, whose warps take turns at the pieces
+  const long rows = a.whole ? 0 : (long)a.B * a.nkv * a.T * a.group;
+  const bool wide = rows > 4L * a.ctas;
+  const long row_blocks = wide ? (rows + JT / 32 - 1) / (JT / 32) : rows;
+  const long blocks = row_blocks + (a.weight ? (long)a.B * a.nkv * ((a.S + a.T + JW - 1) / JW) : 0);
+  if (blocks == 0) return 0;                        // one CTA per unit and no weights: nothing is left to do
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(JT);
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return (int)(wide ? cudaLaunchKernelEx(&cfg, kv_join_k<T, 1>, a, (int)row_blocks)
+                    : cudaLaunchKernelEx(&cfg, kv_join_k<T, JT / 32>, a, (int)row_blocks));
 }
 
 }  // namespace kv

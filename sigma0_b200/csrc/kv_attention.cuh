@@ -38,7 +38,7 @@ S0_DEV int cached(const KvAttnArgs& a, int b) { return min(max(__ldg(a.lengths +
 // key tiles of a sequence: its cached tokens, then the new ones (tiles never mix the two)
 S0_DEV int tiles_of(const KvAttnArgs& a, int len, int KT) { return (len + KT - 1) / KT + (a.T + KT - 1) / KT; }
 
-// s_pre[b] = tiles before sequence b of one (head, row block); returns the total.  Called by all
+// s_pre[b] = tiles of one (head, row block) before sequence b; returns the total.  Called by all
 // threads of the block; needs B + 1 + 32 ints of shared memory.
 S0_DEV long plan_prefix(const KvAttnArgs& a, int KT, int* s_pre) {
   int* s_w = s_pre + a.B + 1;
@@ -102,10 +102,77 @@ S0_DEV Seg find_seg(const KvAttnArgs& a, const int* s_pre, long w, int KT) {
   return s;
 }
 
+// row / group for rows below 2^20: (row + 1/2) / group is at least 1 / (2 group) away from an integer
+S0_DEV int div_group(const KvAttnArgs& a, int row) { return (int)((row + 0.5f) * a.inv_group); }
+
 // the mask row of new token t: which new tokens it sees
+// (indices past the new tokens are clamped, so that the loads need no branch and are in flight together)
 S0_DEV bool sees(const KvAttnArgs& a, int b, int t, int i) {
+  t = min(t, a.T - 1);
+  i = min(i, a.T - 1);
   return a.mask ? a.mask[b * a.mask_b + (long)t * a.T + i] != 0 : i <= t;
 }
+
+// 2^x: results below 2^-126 become 0
+S0_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A unit and the place in it; steps from unit to unit in the plan's order.
+struct Cur {
+  int b, u, len, n, t;  // sequence, head * nrb + row block, cached tokens, tiles, tile
+};
+S0_DEV void cur_set(Cur& c, const KvAttnArgs& a, int KT) {
+  c.len = cached(a, c.b);
+  c.n = tiles_of(a, c.len, KT);
+}
+S0_DEV void cur_next_unit(Cur& c, const KvAttnArgs& a, int KT) {
+  if (++c.u == a.nkv * a.nrb) {
+    c.u = 0;
+    if (++c.b < a.B) cur_set(c, a, KT);
+  }
+}
+// true while the unit stays the same
+S0_DEV bool cur_skip(Cur& c, const KvAttnArgs& a, int KT, int by) {
+  c.t += by;
+  if (c.t < c.n) return true;
+  while (c.b < a.B && c.t >= c.n) {
+    c.t -= c.n;
+    cur_next_unit(c, a, KT);
+  }
+  return false;
+}
+
+// The first tile of this CTA and how many it has.  a.whole: one unit per CTA (caches that are short
+// enough); otherwise the even split, whose prefix table CTA 0 leaves for the join.
+S0_DEV long cta_share(Cur& c, const KvAttnArgs& a, int KT, int* scratch, int ctas) {
+  const int hr = a.nkv * a.nrb;
+  if (a.whole) {
+    c.b = blockIdx.x / hr;
+    c.u = blockIdx.x - c.b * hr;
+    c.t = 0;
+    cur_set(c, a, KT);
+    return c.n;
+  }
+  const Plan p = make_plan(a, plan_prefix(a, KT, scratch), ctas, a.min_per);
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i <= a.B; i += blockDim.x) a.prefix[i] = scratch[i];
+  const long w = (long)blockIdx.x * p.per;
+  if (w >= p.total) return 0;
+  const Seg s = find_seg(a, scratch, w, KT);
+  c.b = s.b;
+  c.u = s.h * a.nrb + s.rb;
+  c.len = s.len;
+  c.n = s.n;
+  c.t = s.t0;
+  return min(p.total - w, p.per);
+}
+
+// Programmatic launch: the joining kernel may be set up while this one runs; it waits for its results.
+S0_DEV void join_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+S0_DEV void join_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // base-2 log-sum-exp of a row; +inf where it saw nothing, so that exp2(s - lse) is 0 there
 S0_DEV float lse2(float m, float l) { return l == 0.f ? CUDART_INF_F : m + log2f(l); }

@@ -2,17 +2,26 @@
 // described in kv_attention.cu; heads up to 128 wide, 16-byte aligned rows).
 //
 // What bounds it: a step reads every cached key and value once and does 4 T group flops per element
-// pair, so up to some 64 rows (new tokens x query heads of a key head) it is bound by HBM.  Both kernels
-// therefore keep a ring of key / value tiles in flight by cp.async all the time, across the ends of
-// units: a CTA's tiles (see kv_attention.cuh) form one stream, and the loads run ahead of the
-// products without regard to which unit a tile belongs to.
-//   kv_attn_few_k    up to 16 rows: every warp streams key slabs of its own (16 keys of 128, 32 of 64
-//                    channels) through its own ring, with a running maximum and sum of its own and no
-//                    barrier; the four warps' results are joined at the end of a unit;
-//   kv_attn_rows_k   more rows: the warps of a CTA take 16 rows each and share the tiles.
-// Products: mma.m16n8k16 with fp32 accumulators.  The scores never leave registers; p is rounded to the
-// cache's type for the second product (relative error u, as the output's own rounding), while the sum
-// of the row is taken from the unrounded values in fp32.
+// pair, so up to some 64 rows (new tokens x query heads of a key head) it is bound by HBM.  A CTA's
+// tiles (see kv_attention.cuh) form one stream, whose loads run ahead by cp.async across the ends of
+// units.
+//
+// The products are transposed: S^T = K Q^T and O^T = V^T P^T with mma.m16n8k16, so that the keys (then
+// the channels) fill the 16 rows of the instruction and the queries its 8 columns.  One token of one
+// head then wastes 7/8 of the products where the usual order wastes 15/16, a warp reads each K and V
+// fragment once for all its 8 NT rows, and the accumulators are half as large.  P^T comes out as
+// accumulators of the first product and goes into the second as its B operand; the two layouts are
+// transposes of one another, which movmatrix turns.
+//   NT  column groups of a warp: 8 or 16 rows;
+//   WR  warps that share a slab of keys for more rows: up to 64 rows in a CTA of four warps.
+// The other warps (4 / WR groups) take slabs of their own, each with a ring, a running maximum and a
+// running sum of its own and no barrier among groups; they are joined at the end of a unit.
+//
+// The maximum that the exponentials refer to moves only when a score passes it by 2^8: the probabilities
+// may be up to 256 instead of 1, which changes no relative error, and the reduction over lanes and the
+// rescaling of the output drop out of nearly every step.  p is rounded to the cache's type for the
+// second product (a relative error of at most the output's own rounding); the sum of the row is taken
+// from the unrounded fp32 values.
 #include <algorithm>
 
 #include "kv_attention.cuh"
@@ -49,221 +58,14 @@ template <typename T> S0_DEV bool any_inf(uint4 x) {
 // consecutive rows fall into eight different groups of banks
 template <int HD> S0_DEV int tile_at(int r, int c) { return r * HD * 2 + ((c ^ (r & 7)) << 4); }
 
-// B fragments of two 8-key groups (rows n0 .. n0 + 15) at channels k0 .. k0 + 15 of a K tile
-template <int HD> S0_DEV void frag_k(uint32_t* f, const char* tile, int n0, int k0, int lane) {
-  const int j = lane >> 3, r = n0 + (lane & 7) + (j >> 1) * 8, c = (k0 >> 3) + (j & 1);
-  ldsm_x4(f[0], f[1], f[2], f[3], tile + tile_at<HD>(r, c));
+S0_DEV uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
-// B fragments of two 8-channel groups (n0 .. n0 + 15) at keys k0 .. k0 + 15 of a V tile
-template <int HD> S0_DEV void frag_v(uint32_t* f, const char* tile, int n0, int k0, int lane) {
-  const int j = lane >> 3, r = k0 + (lane & 7) + (j & 1) * 8, c = (n0 >> 3) + (j >> 1);
-  ldsm_x4_t(f[0], f[1], f[2], f[3], tile + tile_at<HD>(r, c));
-}
-
-// A unit and the place in it; steps from unit to unit in the plan's order.
-struct Cur {
-  int b, u, len, n, t;  // sequence, head * nrb + row block, cached tokens, tiles, tile
-};
-S0_DEV void cur_set(Cur& c, const KvAttnArgs& a, int KT) {
-  c.len = cached(a, c.b);
-  c.n = tiles_of(a, c.len, KT);
-}
-S0_DEV void cur_next_unit(Cur& c, const KvAttnArgs& a, int KT) {
-  if (++c.u == a.nkv * a.nrb) {
-    c.u = 0;
-    if (++c.b < a.B) cur_set(c, a, KT);
-  }
-}
-S0_DEV void cur_skip(Cur& c, const KvAttnArgs& a, int KT, int by) {
-  c.t += by;
-  while (c.b < a.B && c.t >= c.n) {
-    c.t -= c.n;
-    cur_next_unit(c, a, KT);
-  }
-}
-
-// The first tile of this CTA and how many it has.  a.whole: one unit per CTA (caches that are short
-// enough); otherwise the even split.  Leaves the prefix table behind in `scratch` (B + 33 ints).
-S0_DEV long cta_share(Cur& c, const KvAttnArgs& a, int KT, int* scratch, int ctas) {
-  const int hr = a.nkv * a.nrb;
-  if (a.whole) {
-    c.b = blockIdx.x / hr;
-    c.u = blockIdx.x - c.b * hr;
-    c.t = 0;
-    cur_set(c, a, KT);
-    return c.n;
-  }
-  const Plan p = make_plan(a, plan_prefix(a, KT, scratch), ctas, a.min_per);
-  const long w = (long)blockIdx.x * p.per;
-  if (w >= p.total) return 0;
-  const Seg s = find_seg(a, scratch, w, KT);
-  c.b = s.b;
-  c.u = s.h * a.nrb + s.rb;
-  c.len = s.len;
-  c.n = s.n;
-  c.t = s.t0;
-  return min(p.total - w, p.per);
-}
-
-// where row `row` of the unit lies in q / o: element offset of its first channel
-S0_DEV long out_at(const KvAttnArgs& a, int b, int h, int row) {
-  const int t = row / a.group, g = row - t * a.group;
-  return (((long)b * a.T + t) * a.nkv * a.group + h * a.group + g) * a.hd;
-}
-template <typename T> S0_DEV const T* q_at(const KvAttnArgs& a, int b, int h, int row) {
-  const int t = row / a.group, g = row - t * a.group;
-  return (const T*)a.q + b * a.q_b + t * a.q_t + (long)(h * a.group + g) * a.q_h;
-}
-
-// A fragments of rows [r0, r0 + 16) straight from global memory; rows past R and channels past hd are 0
-template <typename T, int HD>
-S0_DEV void load_q(uint32_t (*qf)[4], const KvAttnArgs& a, int b, int h, int r0, int R, int lane) {
-  const int g = lane >> 2, t = lane & 3;
-  const T* p0 = r0 + g < R ? q_at<T>(a, b, h, r0 + g) : nullptr;
-  const T* p1 = r0 + g + 8 < R ? q_at<T>(a, b, h, r0 + g + 8) : nullptr;
-#pragma unroll
-  for (int k = 0; k < HD / 16; ++k)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const T* p = e & 1 ? p1 : p0;
-      const int d = k * 16 + (e >> 1) * 8 + 2 * t;
-      qf[k][e] = p && d < a.hd ? *reinterpret_cast<const uint32_t*>(p + d) : 0u;
-    }
-}
-
-// A tile of new tokens: hidden rows' NaNs and infinities must not meet their zero probabilities in the
-// product, so what is not finite in V is added by hand to the rows that see it, and taken out of the
-// tile.  `own(e)`: this thread's rows; NK keys.  Rare: only tiles that hold such a value come here.
+// stores a slab of new rows behind the cached ones
 template <typename T, int HD, int NK>
-S0_DEV void add_infinities(float (*o)[4], char* tv, const KvAttnArgs& a, int b, int row0, int R, int k0, int nk, int lane) {
-  const int g = lane >> 2, t = lane & 3;
-  for (int j = 0; j < nk; ++j)
-#pragma unroll
-    for (int nt = 0; nt < HD / 8; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int row = row0 + g + (e >> 1) * 8, d = nt * 8 + 2 * t + (e & 1);
-        const unsigned short x = *reinterpret_cast<const unsigned short*>(tv + tile_at<HD>(j, nt) + (2 * t + (e & 1)) * 2);
-        if ((x & Inf<T>::mask) == Inf<T>::mask && row < R && d < a.hd && sees(a, b, row / a.group, k0 + j))
-          o[nt][e] += Elem<T>::to(*reinterpret_cast<const T*>(&x));
-      }
-}
-template <typename T, int HD, int NK>
-S0_DEV void drop_infinities(char* tv, int i0, int step) {
-  for (int i = i0; i < NK * HD; i += step) {
-    const int j = i / HD, d = i - j * HD;
-    unsigned short* p = reinterpret_cast<unsigned short*>(tv + tile_at<HD>(j, d >> 3) + (d & 7) * 2);
-    if ((*p & Inf<T>::mask) == Inf<T>::mask) *p = 0;
-  }
-}
-
-// Softmax of a warp's 16 x NK scores in place, with the running statistics and the rescaled output.
-// Rows g and g + 8 of the block at row0; keys k0 + ... of which nk exist.
-template <typename T, int HD, int NK>
-S0_DEV void softmax_tile(float (*s)[4], float (*o)[4], float* m, float* l, const KvAttnArgs& a, int b, long bh, int row0,
-                         int R, bool tail, int len, int k0, int nk, int lane) {
-  const int g = lane >> 2, t = lane & 3;
-  const bool part = tail || nk < NK;
-#pragma unroll
-  for (int nt = 0; nt < NK / 8; ++nt)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float x = s[nt][e] * a.scale_log2;
-      if (part) {
-        const int j = nt * 8 + 2 * t + (e & 1), row = row0 + g + (e >> 1) * 8;
-        if (j >= nk || (tail && (row >= R || !sees(a, b, row / a.group, k0 + j)))) x = -CUDART_INF_F;
-      }
-      s[nt][e] = x;
-    }
-  if (a.scores) {
-#pragma unroll
-    for (int nt = 0; nt < NK / 8; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = nt * 8 + 2 * t + (e & 1), row = row0 + g + (e >> 1) * 8;
-        if (j < nk && row < R) a.scores[(bh * R + row) * a.sp + (tail ? len : 0) + k0 + j] = s[nt][e];
-      }
-  }
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    float mx = m[r];
-#pragma unroll
-    for (int nt = 0; nt < NK / 8; ++nt) mx = fmaxf(mx, fmaxf(s[nt][2 * r], s[nt][2 * r + 1]));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    const float base = mx == -CUDART_INF_F ? 0.f : mx;   // a row that has seen nothing yet
-    const float al = exp2f(m[r] - base);
-    m[r] = mx;
-    float sum = 0.f;
-#pragma unroll
-    for (int nt = 0; nt < NK / 8; ++nt) {
-      s[nt][2 * r] = exp2f(s[nt][2 * r] - base);
-      s[nt][2 * r + 1] = exp2f(s[nt][2 * r + 1] - base);
-      sum += s[nt][2 * r] + s[nt][2 * r + 1];
-    }
-    l[r] = l[r] * al + sum;                              // this lane's share; joined at the end
-#pragma unroll
-    for (int i = 0; i < HD / 8; ++i) {
-      o[i][2 * r] *= al;
-      o[i][2 * r + 1] *= al;
-    }
-  }
-}
-
-// a finished unit's or a piece's rows from the accumulators
-template <typename T, int HD>
-S0_DEV void write_rows(float (*o)[4], const float* m, const float* l, const KvAttnArgs& a, int b, int h, int r0, int row0, int R,
-                       bool all, long slot, int lane) {
-  const int g = lane >> 2, t = lane & 3;
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int row = row0 + g + 8 * r;
-    if (row >= R) continue;
-    if (all) {
-      const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
-      T* p = (T*)a.o + out_at(a, b, h, row);
-#pragma unroll
-      for (int nt = 0; nt < HD / 8; ++nt)
-        if (nt * 8 < a.hd)
-          *reinterpret_cast<uint32_t*>(p + nt * 8 + 2 * t) = pack2<T>(o[nt][2 * r] * inv, o[nt][2 * r + 1] * inv);
-      if (a.lse && t == 0) a.lse[((long)b * a.nkv + h) * R + row] = lse2(m[r], l[r]);
-    } else {
-      const long at = slot * a.rows + row - r0;
-#pragma unroll
-      for (int nt = 0; nt < HD / 8; ++nt)
-        if (nt * 8 < a.hd)
-          *reinterpret_cast<float2*>(a.part_o + at * a.hd + nt * 8 + 2 * t) = make_float2(o[nt][2 * r], o[nt][2 * r + 1]);
-      if (t == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m[r], l[r]);
-    }
-  }
-}
-
-// One tile of a unit's stream into a stage: K rows, then V rows; what does not exist becomes 0.
-template <typename T, int HD, int NK, int NT>
-S0_DEV void load_tile(char* st, const KvAttnArgs& a, const Cur& c, int tid) {
-  constexpr int C = HD / 8, RS = NT / C;               // chunks of a row, rows per pass
-  const int ncache = (c.len + NK - 1) / NK, h = c.u / a.nrb;
-  const bool tail = c.t >= ncache;
-  const int k0 = (tail ? c.t - ncache : c.t) * NK, nk = (tail ? a.T : c.len) - k0;
-  const int ch = tid % C, r0 = tid / C;
-  const long ks = tail ? a.kn_t : a.kc_s, vs = tail ? a.vn_t : a.vc_s;
-  const T* k = tail ? (const T*)a.kn + c.b * a.kn_b + h * a.kn_h : (const T*)a.kc + c.b * a.kc_b + h * a.kc_h;
-  const T* v = tail ? (const T*)a.vn + c.b * a.vn_b + h * a.vn_h : (const T*)a.vc + c.b * a.vc_b + h * a.vc_h;
-  const bool in = ch * 8 < a.hd;
-  k += (in ? ch * 8 : 0) + (k0 + r0) * ks;
-  v += (in ? ch * 8 : 0) + (k0 + r0) * vs;
-#pragma unroll
-  for (int i = 0; i < NK / RS; ++i) {
-    const int r = r0 + i * RS;
-    const bool ok = in && r < nk;
-    cp_async16(st + tile_at<HD>(r, ch), ok ? k + (long)i * RS * ks : a.q, ok ? 16 : 0);
-    cp_async16(st + NK * HD * 2 + tile_at<HD>(r, ch), ok ? v + (long)i * RS * vs : a.q, ok ? 16 : 0);
-  }
-}
-
-// stores a tile of new rows behind the cached ones
-template <typename T, int HD, int NK>
-S0_DEV void put_tile(const char* st, const KvAttnArgs& a, int b, int h, int len, int k0, int nk, int i0, int step) {
+S0_DEV void put_slab(const char* st, const KvAttnArgs& a, int b, int h, int len, int k0, int nk, int i0, int step) {
   const int C = a.hd / 8;
   for (int i = i0; i < nk * C; i += step) {
     const int r = i / C, ch = i - r * C;
@@ -279,156 +81,372 @@ S0_DEV void put_tile(const char* st, const KvAttnArgs& a, int b, int h, int len,
       if (len + k0 + r < a.S) a.positions[b * a.pos_b + h * a.pos_h + len + k0 + r] = a.seen[b] + k0 + r;
 }
 
-constexpr int FW = 4, FS = 3;  // warps of a block, stages of a warp's ring
+constexpr int WARPS = 4, SLAB = 8192;   // warps, bytes of K and V per warp and stage
 
-template <int HD> constexpr int few_keys() { return HD == 128 ? 16 : 32; }
-template <int HD> constexpr int few_stage() { return 2 * few_keys<HD>() * HD * 2; }
+// stages of a ring and CTAs of an SM: 64 rows are a longer chain of products per slab and want more warps,
+// fewer rows more bytes in flight per warp
+template <int WR> constexpr int stages() { return WR == WARPS ? 2 : 3; }
+template <int WR> constexpr int per_sm() { return WR == WARPS ? 3 : 2; }
+template <int HD, int WR> constexpr int slab_keys() { return SLAB * WR / (HD * 4); }
+// accumulators in passing: 2 warps (groups 2, 3 -> 0, 1) or WR warps (group 1 -> 0) at a time, maxima and sums
+template <int HD, int NT, int WR> constexpr int join_bytes() {
+  return WR == WARPS ? 0 : 2 * (HD / 16 * NT * 4 * 128 + NT * 8 * 2 * 4);
+}
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(32 * FW, 2) kv_attn_few_k(KvAttnArgs a, int ctas) {
-  constexpr int NK = few_keys<HD>(), SB = few_stage<HD>(), OLD = HD + 4;
+template <int N> S0_DEV void group_sync(int group) {
+  if constexpr (N == 1) __syncwarp();
+  else if constexpr (N == WARPS) __syncthreads();
+  else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(32 * N) : "memory");
+}
+
+template <typename T, int HD, int NT, int WR>
+__global__ void __launch_bounds__(32 * WARPS, per_sm<WR>()) kv_attn_tc_k(KvAttnArgs a, int ctas) {
+  constexpr int NK = slab_keys<HD, WR>(), WK = WARPS / WR, SB = SLAB * WR, NTH = 32 * WR, STAGES = stages<WR>();
+  constexpr int KG = NK % 32 == 0 ? 2 : 1;                      // groups of 16 keys in flight at once
+  constexpr int C = HD / 8, RS = NTH / C;                       // 16-byte chunks of a row, rows of a loading pass
   extern __shared__ __align__(128) char smem[];
+  join_may_start();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int R = a.T * a.group, mrows = min(16, R);
-  char* ring = smem + warp * FS * SB;
-  float* sO = reinterpret_cast<float*>(smem + FW * FS * SB);   // [2][mrows][OLD] outputs of two warps
-  float* sM = sO + 2 * mrows * OLD;                            // [2][mrows][2] maxima, sums
+  const int group = warp / WR, wr = warp % WR, gt = tid - group * NTH;
+  const int R = a.T * a.group;
+  char* ring = smem + group * STAGES * SB;
+  float* sJ = reinterpret_cast<float*>(smem + WK * STAGES * SB);
   Cur cur;
   const long share = cta_share(cur, a, NK, reinterpret_cast<int*>(smem), ctas);
-  __syncthreads();                                             // the plan's scratch becomes the ring
+  __syncthreads();                                              // the plan's scratch becomes the rings
   if (share <= 0) return;
 
-  Cur ahead = cur;                                             // this warp's next tile to load
-  long left = (share - warp + FW - 1) / FW;
-  cur_skip(ahead, a, NK, warp);
+  // ---- loading: this group's slabs of the share, ahead of their use -------------------------------
+  Cur ahead = cur;
+  int left = (int)((share - group + WK - 1) / WK);
+  const int ch = gt % C, lr = gt / C;                           // this thread's chunk and first row
+  const bool in = ch * 8 < a.hd;
+  const char *kp = nullptr, *vp = nullptr;                      // its first row's addresses in the slab
+  long ks = 0, vs = 0;                                          // bytes from pass to pass
+  int rows = 0;                                                 // rows of the source from the slab on
+  bool fresh = false;                                           // the source is the new tokens
+  auto aim = [&]() {
+    const int ncache = (ahead.len + NK - 1) / NK, h = ahead.u / a.nrb;
+    const bool tail = fresh = ahead.t >= ncache;
+    const int k0 = (tail ? ahead.t - ncache : ahead.t) * NK;
+    rows = (tail ? a.T : ahead.len) - k0;
+    const long k1 = tail ? a.kn_t : a.kc_s, v1 = tail ? a.vn_t : a.vc_s;
+    const T* k = tail ? (const T*)a.kn + ahead.b * a.kn_b + h * a.kn_h : (const T*)a.kc + ahead.b * a.kc_b + h * a.kc_h;
+    const T* v = tail ? (const T*)a.vn + ahead.b * a.vn_b + h * a.vn_h : (const T*)a.vc + ahead.b * a.vc_b + h * a.vc_h;
+    kp = reinterpret_cast<const char*>(k + (k0 + lr) * k1 + ch * 8);
+    vp = reinterpret_cast<const char*>(v + (k0 + lr) * v1 + ch * 8);
+    ks = k1 * (RS * 2);
+    vs = v1 * (RS * 2);
+  };
   auto fetch = [&](int stage) {
     if (left > 0) {
-      load_tile<T, HD, NK, 32>(ring + stage * SB, a, ahead, lane);
-      if (--left > 0) cur_skip(ahead, a, NK, FW);
+      char* st = ring + stage * SB + tile_at<HD>(lr, ch);
+      const bool full = rows >= NK && a.hd == HD;
+#pragma unroll
+      for (int i = 0; i < NK / RS; ++i) {
+        char* d = RS % 8 == 0 ? st + i * RS * HD * 2 : ring + stage * SB + tile_at<HD>(lr + i * RS, ch);
+        const bool ok = full || (in && lr + i * RS < rows);
+        cp_async16(d, ok ? kp + i * ks : (const char*)a.q, ok ? 16 : 0);
+        cp_async16(d + NK * HD * 2, ok ? vp + i * vs : (const char*)a.q, ok ? 16 : 0);
+      }
+      if (--left > 0) {
+        if (cur_skip(ahead, a, NK, WK) && !fresh && rows > WK * NK) {
+          kp += ks * (WK * NK / RS);
+          vp += vs * (WK * NK / RS);
+          rows -= WK * NK;
+        } else {
+          aim();
+        }
+      }
     }
     cp_async_commit();
   };
+  if (left > 0) {
+    cur_skip(ahead, a, NK, group);
+    aim();
+  }
 #pragma unroll
-  for (int i = 0; i < FS - 1; ++i) fetch(i);
+  for (int i = 0; i < STAGES - 1; ++i) fetch(i);
 
-  long done = 0;                                               // tiles of the share before this unit
+  // ---- the units of the share ---------------------------------------------------------------------
+  long done = 0, mine = group;                                  // tiles before this unit, this group's next
   int stage = 0;
-  long mine = warp;                                            // this warp's next tile of the share
   while (done < share) {
-    const int b = cur.b, h = cur.u / a.nrb, rb = cur.u - h * a.nrb, r0 = rb * 16;
+    const int b = cur.b, h = cur.u / a.nrb, rb = cur.u - h * a.nrb, r0 = rb * a.rows, row0 = r0 + wr * 8 * NT;
     const long bh = (long)b * a.nkv + h;
     const int t1 = (int)min((long)cur.n, cur.t + (share - done));
     const int ncache = (cur.len + NK - 1) / NK;
     const long end = done + (t1 - cur.t);
-    uint32_t qf[HD / 16][4];
-    load_q<T, HD>(qf, a, b, h, r0, R, lane);
-    float o[HD / 8][4];
+    // B fragments of Q^T: rows row0 + 8 nt + g
+    uint32_t qf[NT][HD / 16][2];
 #pragma unroll
-    for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = row0 + 8 * nt + g, tok = div_group(a, row);
+      const T* p = (const T*)a.q + b * a.q_b + tok * a.q_t + (long)(h * a.group + row - tok * a.group) * a.q_h;
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int d = k * 16 + e * 8 + 2 * t;
+          qf[nt][k][e] = row < R && d < a.hd ? *reinterpret_cast<const uint32_t*>(p + d) : 0u;
+        }
+    }
+    float o[HD / 16][NT][4];                                    // channels 16 mt + g (+ 8), rows 8 nt + 2 t (+ 1)
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = -CUDART_INF_F;
+      l[nt][0] = l[nt][1] = 0.f;                                // this lane's keys only, until the end
+    }
 
-    for (; mine < end; mine += FW) {
+    for (; mine < end; mine += WK) {
       const int tt = cur.t + (int)(mine - done);
-      __syncwarp();                                            // the stage that is loaded next has been read
-      fetch(stage == 0 ? FS - 1 : stage - 1);
-      cp_async_wait_group<FS - 1>();
-      __syncwarp();
-      char* st = ring + stage * SB;
+      cp_async_wait_group<STAGES - 2>();
+      group_sync<WR>(group);                                    // the slab is there, the one before it has been read
+      fetch(stage == 0 ? STAGES - 1 : stage - 1);
+      char* sk = ring + stage * SB;
+      char* sv = sk + NK * HD * 2;
       const bool tail = tt >= ncache;
       const int k0 = (tail ? tt - ncache : tt) * NK, nk = min(NK, (tail ? a.T : cur.len) - k0);
-      float s[NK / 8][4];
-#pragma unroll
-      for (int i = 0; i < NK / 8; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
-#pragma unroll
-      for (int kk = 0; kk < HD / 16; ++kk)
-#pragma unroll
-        for (int np = 0; np < NK / 16; ++np) {
-          uint32_t f[4];
-          frag_k<HD>(f, st, np * 16, kk * 16, lane);
-          mma16<T>(s[2 * np], qf[kk], f[0], f[1]);
-          mma16<T>(s[2 * np + 1], qf[kk], f[2], f[3]);
-        }
-      softmax_tile<T, HD, NK>(s, o, m, l, a, b, bh, r0, R, tail, cur.len, k0, nk, lane);
-      char* tv = st + NK * HD * 2;
+      // A hidden row's NaN or infinity must not meet its zero probability in the product: what is not finite
+      // in V is taken out of the slab, and added by hand, after the product, to the rows that see it.
+      bool bad = false;
       if (tail) {
-        if (rb == 0) put_tile<T, HD, NK>(st, a, b, h, cur.len, k0, nk, lane, 32);
-        bool bad = false;
-        for (int i = lane; i < NK * HD / 8; i += 32) bad |= any_inf<T>(*reinterpret_cast<const uint4*>(tv + i * 16));
-        if (__any_sync(0xffffffffu, bad)) {
-          add_infinities<T, HD, NK>(o, tv, a, b, r0, R, k0, nk, lane);
-          __syncwarp();
-          drop_infinities<T, HD, NK>(tv, lane, 32);
-          __syncwarp();
+        if (rb == 0) put_slab<T, HD, NK>(sk, a, b, h, cur.len, k0, nk, gt, NTH);
+        for (int i = lane; i < NK * C; i += 32) bad |= any_inf<T>(*reinterpret_cast<const uint4*>(sv + i * 16));
+        bad = __any_sync(0xffffffffu, bad);
+        if (bad) {
+          group_sync<WR>(group);
+          for (int i = gt; i < NK * HD; i += NTH) {
+            unsigned short* p = reinterpret_cast<unsigned short*>(sv + tile_at<HD>(i / HD, (i % HD) >> 3) + (i & 7) * 2);
+            if ((*p & Inf<T>::mask) == Inf<T>::mask) *p = 0;
+          }
+          group_sync<WR>(group);
         }
       }
+#pragma unroll 1
+      for (int kk = 0; kk < NK; kk += 16 * KG) {
+        if (kk >= nk) break;
+        // S^T of 16 KG keys: rows kk + 16 q + g (+ 8), columns 8 nt + 2 t (+ 1)
+        float s[KG][NT][4];
 #pragma unroll
-      for (int kk = 0; kk < NK / 16; ++kk) {
-        uint32_t pa[4];
-        pa[0] = pack2<T>(s[2 * kk][0], s[2 * kk][1]);
-        pa[1] = pack2<T>(s[2 * kk][2], s[2 * kk][3]);
-        pa[2] = pack2<T>(s[2 * kk + 1][0], s[2 * kk + 1][1]);
-        pa[3] = pack2<T>(s[2 * kk + 1][2], s[2 * kk + 1][3]);
+        for (int q = 0; q < KG; ++q)
 #pragma unroll
-        for (int dp = 0; dp < HD / 16; ++dp) {
-          uint32_t f[4];
-          frag_v<HD>(f, tv, dp * 16, kk * 16, lane);
-          mma16<T>(o[2 * dp], pa, f[0], f[1]);
-          mma16<T>(o[2 * dp + 1], pa, f[2], f[3]);
+          for (int nt = 0; nt < NT; ++nt) s[q][nt][0] = s[q][nt][1] = s[q][nt][2] = s[q][nt][3] = 0.f;
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+          for (int q = 0; q < KG; ++q) {
+            uint32_t f[4];                                      // A: 16 keys x 16 channels
+            ldsm_x4(f[0], f[1], f[2], f[3], sk + tile_at<HD>(kk + 16 * q + (lane & 15), 2 * k + (lane >> 4)));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16<T>(s[q][nt], f, qf[nt][k][0], qf[nt][k][1]);
+          }
+        if (kk + 16 * KG > nk || tail) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int row = row0 + 8 * nt + 2 * t + e, tok = div_group(a, row);
+#pragma unroll
+              for (int q = 0; q < KG; ++q)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                  const int j = kk + 16 * q + g + 8 * x;
+                  bool vis = j < nk;
+                  if (tail) vis &= (row < R) & sees(a, b, tok, k0 + j);
+                  if (!vis) s[q][nt][2 * x + e] = -CUDART_INF_F;
+                }
+            }
+        }
+        if (a.scores) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int row = row0 + 8 * nt + 2 * t + e;
+              if (row < R) {
+                float* p = a.scores + (bh * R + row) * a.sp + (tail ? cur.len : 0) + k0 + kk + g;
+#pragma unroll
+                for (int q = 0; q < KG; ++q)
+#pragma unroll
+                  for (int x = 0; x < 2; ++x)
+                    if (kk + 16 * q + g + 8 * x < nk) p[16 * q + 8 * x] = s[q][nt][2 * x + e] * a.scale_log2;
+              }
+            }
+        }
+        // does a score pass its row's reference by 2^8?
+        float mx[NT][2];
+        bool far = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
+#pragma unroll
+            for (int q = 1; q < KG; ++q) x = fmaxf(x, fmaxf(s[q][nt][e], s[q][nt][2 + e]));
+            mx[nt][e] = x * a.scale_log2;
+            far |= mx[nt][e] > m[nt][e] + 8.f;
+          }
+        if (__any_sync(0xffffffffu, far)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float x = fmaxf(mx[nt][e], m[nt][e]);
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+              const float al = x == -CUDART_INF_F ? 1.f : ex2(m[nt][e] - x);
+              m[nt][e] = x;
+              l[nt][e] *= al;
+#pragma unroll
+              for (int i = 0; i < HD / 16; ++i) {
+                o[i][nt][e] *= al;
+                o[i][nt][2 + e] *= al;
+              }
+            }
+        }
+        uint32_t pf[KG][NT][2];                                 // B: 16 keys x 8 rows
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float b0 = m[nt][0] == -CUDART_INF_F ? 0.f : m[nt][0], b1 = m[nt][1] == -CUDART_INF_F ? 0.f : m[nt][1];
+#pragma unroll
+          for (int q = 0; q < KG; ++q)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const float p0 = ex2(fmaf(s[q][nt][2 * x], a.scale_log2, -b0));
+              const float p1 = ex2(fmaf(s[q][nt][2 * x + 1], a.scale_log2, -b1));
+              l[nt][0] += p0;
+              l[nt][1] += p1;
+              pf[q][nt][x] = transpose8(pack2<T>(p0, p1));
+            }
+        }
+        // O^T += V^T P^T
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+          for (int q = 0; q < KG; ++q) {
+            uint32_t f[4];                                      // A: 16 channels x 16 keys, V read transposed
+            ldsm_x4_t(f[0], f[1], f[2], f[3],
+                      sv + tile_at<HD>(kk + 16 * q + (lane & 7) + (lane >> 4) * 8, 2 * i + ((lane >> 3) & 1)));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16<T>(o[i][nt], f, pf[q][nt][0], pf[q][nt][1]);
+          }
+      }
+      if (bad) {
+        const T* vn = (const T*)a.vn + b * a.vn_b + h * a.vn_h;
+        for (int j = 0; j < nk; ++j) {
+          uint32_t vis = 0;
+#pragma unroll
+          for (int i = 0; i < 2 * NT; ++i) {
+            const int row = row0 + (i >> 1) * 8 + 2 * t + (i & 1);
+            if (row < R && sees(a, b, div_group(a, row), k0 + j)) vis |= 1u << i;
+          }
+#pragma unroll
+          for (int i = 0; i < HD / 8; ++i) {
+            if (i * 8 >= a.hd) break;
+            const float v = Elem<T>::to(vn[(k0 + j) * a.vn_t + i * 8 + g]);
+            if (isfinite(v)) continue;
+#pragma unroll
+            for (int r = 0; r < 2 * NT; ++r)
+              if (vis >> r & 1) o[i >> 1][r >> 1][(i & 1) * 2 + (r & 1)] += v;
+          }
         }
       }
-      stage = stage == FS - 1 ? 0 : stage + 1;
+      stage = stage == STAGES - 1 ? 0 : stage + 1;
     }
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    }
-    // join the warps: 2 and 3 hand over to 0 and 1, then 1 to 0
-    auto give = [&](int slot) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = g + 8 * r;
-        if (row >= mrows) continue;
-        float* p = sO + (slot * mrows + row) * OLD + 2 * t;
-#pragma unroll
-        for (int nt = 0; nt < HD / 8; ++nt) *reinterpret_cast<float2*>(p + nt * 8) = make_float2(o[nt][2 * r], o[nt][2 * r + 1]);
-        if (t == 0) {
-          sM[(slot * mrows + row) * 2] = m[r];
-          sM[(slot * mrows + row) * 2 + 1] = l[r];
-        }
+      for (int e = 0; e < 2; ++e) {
+        l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 4);
+        l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 8);
+        l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 16);
       }
-    };
-    auto take = [&](int slot) {
+
+    // ---- join the groups: 2 and 3 hand over to 0 and 1, then 1 to 0 -------------------------------
+    if constexpr (WK > 1) {
+      constexpr int MT = HD / 16, PER = MT * NT * 4 * 32;
+      float* sM = sJ + 2 * PER;                                 // [2][8 NT][2]
+      auto give = [&](int slot) {
+        float* buf = sJ + slot * PER + lane;
+        float* ml = sM + slot * NT * 16 + 4 * t;                // rows 2 t, 2 t + 1 of a column group
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = g + 8 * r;
-        if (row >= mrows) continue;
-        const float m2 = sM[(slot * mrows + row) * 2], l2 = sM[(slot * mrows + row) * 2 + 1];
-        const float mx = fmaxf(m[r], m2), base = mx == -CUDART_INF_F ? 0.f : mx;
-        const float e0 = exp2f(m[r] - base), e1 = exp2f(m2 - base);
-        m[r] = mx;
-        l[r] = l[r] * e0 + l2 * e1;
-        const float* p = sO + (slot * mrows + row) * OLD + 2 * t;
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int nt = 0; nt < HD / 8; ++nt) {
-          const float2 x = *reinterpret_cast<const float2*>(p + nt * 8);
-          o[nt][2 * r] = o[nt][2 * r] * e0 + x.x * e1;
-          o[nt][2 * r + 1] = o[nt][2 * r + 1] * e0 + x.y * e1;
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) buf[((i * NT + nt) * 4 + e) * 32] = o[i][nt][e];
+        if (g == 0) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            *reinterpret_cast<float4*>(ml + nt * 16) = make_float4(m[nt][0], l[nt][0], m[nt][1], l[nt][1]);
         }
+      };
+      auto take = [&](int slot) {
+        const float* buf = sJ + slot * PER + lane;
+        const float* ml = sM + slot * NT * 16 + 4 * t;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float m2 = ml[nt * 16 + 2 * e], x = fmaxf(m[nt][e], m2);
+            const float e0 = x == -CUDART_INF_F ? 1.f : ex2(m[nt][e] - x), e1 = x == -CUDART_INF_F ? 0.f : ex2(m2 - x);
+            m[nt][e] = x;
+            l[nt][e] = l[nt][e] * e0 + ml[nt * 16 + 2 * e + 1] * e1;
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+              for (int y = 0; y < 2; ++y)
+                o[i][nt][2 * y + e] = o[i][nt][2 * y + e] * e0 + buf[((i * NT + nt) * 4 + 2 * y + e) * 32] * e1;
+          }
+      };
+      if constexpr (WK == 4) {
+        if (warp >= 2) give(warp - 2);
+        __syncthreads();
+        if (warp < 2) take(warp);
+        __syncwarp();
+        if (warp == 1) give(1);                                 // only this warp has read slot 1
+        __syncthreads();
+        if (warp == 0) take(1);                                 // slot 0 is free from here, slot 1 after the next barrier
+      } else {
+        if (group == 1) give(wr);
+        __syncthreads();
+        if (group == 0) take(wr);
+        __syncthreads();
       }
-    };
-    if (warp >= 2) give(warp - 2);
-    __syncthreads();
-    if (warp < 2) take(warp);
-    if (warp == 1) {
-      __syncwarp();
-      give(1);                                                 // slot 1 is read by this warp only
     }
-    __syncthreads();
-    if (warp == 0) {
-      take(1);
+    if (group == 0) {
       const bool first = cur.t == 0, all = first && t1 == cur.n;
-      write_rows<T, HD>(o, m, l, a, b, h, r0, r0, R, all, 2L * blockIdx.x + (first ? 1 : 0), lane);
+      const long slot = 2L * blockIdx.x + (first ? 1 : 0);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = row0 + 8 * nt + 2 * t + e;
+          if (row >= R) continue;
+          if (all) {
+            const int tok = div_group(a, row);
+            const float inv = l[nt][e] == 0.f ? 0.f : 1.f / l[nt][e];
+            T* p = (T*)a.o + (((long)b * a.T + tok) * a.nkv * a.group + h * a.group + row - tok * a.group) * a.hd + g;
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i)
+              if (i * 8 < a.hd) p[i * 8] = Elem<T>::of(o[i >> 1][nt][(i & 1) * 2 + e] * inv);
+            if (a.lse && g == 0) a.lse[bh * R + row] = lse2(m[nt][e], l[nt][e]);
+          } else {
+            const long at = slot * a.rows + row - r0;
+            float* p = a.part_o + at * a.hd + g;
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i)
+              if (i * 8 < a.hd) p[i * 8] = o[i >> 1][nt][(i & 1) * 2 + e];
+            if (g == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m[nt][e], l[nt][e]);
+          }
+        }
     }
     done = end;
     cur.t = 0;
@@ -436,127 +454,23 @@ __global__ void __launch_bounds__(32 * FW, 2) kv_attn_few_k(KvAttnArgs a, int ct
   }
 }
 
-// WR warps of 16 rows each
-template <int HD> constexpr int rows_keys() { return 64; }
-
-template <typename T, int HD, int WR, int ST>
-__global__ void __launch_bounds__(32 * WR, WR == 8 ? 1 : 2) kv_attn_rows_k(KvAttnArgs a, int ctas) {
-  constexpr int NK = rows_keys<HD>(), SB = 2 * NK * HD * 2, NT = 32 * WR;
-  extern __shared__ __align__(128) char smem[];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int R = a.T * a.group;
-  Cur cur;
-  const long share = cta_share(cur, a, NK, reinterpret_cast<int*>(smem), ctas);
-  __syncthreads();
-  if (share <= 0) return;
-  Cur ahead = cur;
-  long left = share;
-  auto fetch = [&](int stage) {
-    if (left > 0) {
-      load_tile<T, HD, NK, NT>(smem + stage * SB, a, ahead, tid);
-      if (--left > 0) cur_skip(ahead, a, NK, 1);
-    }
-    cp_async_commit();
-  };
-#pragma unroll
-  for (int i = 0; i < ST - 1; ++i) fetch(i);
-
-  long done = 0;
-  int stage = 0;
-  while (done < share) {
-    const int b = cur.b, h = cur.u / a.nrb, rb = cur.u - h * a.nrb, r0 = rb * 16 * WR, row0 = r0 + 16 * warp;
-    const long bh = (long)b * a.nkv + h;
-    const int t1 = (int)min((long)cur.n, cur.t + (share - done));
-    const int ncache = (cur.len + NK - 1) / NK;
-    uint32_t qf[HD / 16][4];
-    load_q<T, HD>(qf, a, b, h, row0, R, lane);
-    float o[HD / 8][4];
-#pragma unroll
-    for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
-    for (int tt = cur.t; tt < t1; ++tt) {
-      cp_async_wait_group<ST - 2>();
-      __syncthreads();                                         // the tile is there, and the one before it has been read
-      fetch(stage == 0 ? ST - 1 : stage - 1);
-      char* st = smem + stage * SB;
-      char* tv = st + NK * HD * 2;
-      const bool tail = tt >= ncache;
-      const int k0 = (tail ? tt - ncache : tt) * NK, nk = min(NK, (tail ? a.T : cur.len) - k0);
-      float s[NK / 8][4];
-#pragma unroll
-      for (int i = 0; i < NK / 8; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
-#pragma unroll
-      for (int kk = 0; kk < HD / 16; ++kk)
-#pragma unroll
-        for (int np = 0; np < NK / 16; ++np) {
-          uint32_t f[4];
-          frag_k<HD>(f, st, np * 16, kk * 16, lane);
-          mma16<T>(s[2 * np], qf[kk], f[0], f[1]);
-          mma16<T>(s[2 * np + 1], qf[kk], f[2], f[3]);
-        }
-      softmax_tile<T, HD, NK>(s, o, m, l, a, b, bh, row0, R, tail, cur.len, k0, nk, lane);
-      if (tail) {
-        if (rb == 0) put_tile<T, HD, NK>(st, a, b, h, cur.len, k0, nk, tid, NT);
-        bool bad = false;
-        for (int i = tid; i < NK * HD / 8; i += NT) bad |= any_inf<T>(*reinterpret_cast<const uint4*>(tv + i * 16));
-        if (__syncthreads_or(bad)) {
-          add_infinities<T, HD, NK>(o, tv, a, b, row0, R, k0, nk, lane);
-          __syncthreads();
-          drop_infinities<T, HD, NK>(tv, tid, NT);
-          __syncthreads();
-        }
-      }
-#pragma unroll
-      for (int kk = 0; kk < NK / 16; ++kk) {
-        uint32_t pa[4];
-        pa[0] = pack2<T>(s[2 * kk][0], s[2 * kk][1]);
-        pa[1] = pack2<T>(s[2 * kk][2], s[2 * kk][3]);
-        pa[2] = pack2<T>(s[2 * kk + 1][0], s[2 * kk + 1][1]);
-        pa[3] = pack2<T>(s[2 * kk + 1][2], s[2 * kk + 1][3]);
-#pragma unroll
-        for (int dp = 0; dp < HD / 16; ++dp) {
-          uint32_t f[4];
-          frag_v<HD>(f, tv, dp * 16, kk * 16, lane);
-          mma16<T>(o[2 * dp], pa, f[0], f[1]);
-          mma16<T>(o[2 * dp + 1], pa, f[2], f[3]);
-        }
-      }
-      stage = stage == ST - 1 ? 0 : stage + 1;
-    }
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    }
-    const bool first = cur.t == 0, all = first && t1 == cur.n;
-    write_rows<T, HD>(o, m, l, a, b, h, r0, row0, R, all, 2L * blockIdx.x + (first ? 1 : 0), lane);
-    done += t1 - cur.t;
-    cur.t = 0;
-    cur_next_unit(cur, a, NK);
-  }
-}
-
-template <typename K>
-int run_k(K k, const KvAttnArgs& a, int threads, size_t sm, cudaStream_t st) {
-  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
+template <typename T, int HD, int NT, int WR>
+int run_tc(const KvAttnArgs& a, cudaStream_t st) {
+  const size_t sm = std::max<size_t>(WARPS * stages<WR>() * SLAB + join_bytes<HD, NT, WR>(), (size_t)(a.B + 33) * 4);
+  const cudaError_t e = cudaFuncSetAttribute(kv_attn_tc_k<T, HD, NT, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
   if (e != cudaSuccess) return (int)e;
-  const int grid = a.whole ? a.B * a.nkv * a.nrb : a.ctas;
-  k<<<grid, threads, sm, st>>>(a, a.ctas);
+  kv_attn_tc_k<T, HD, NT, WR><<<a.whole ? a.B * a.nkv * a.nrb : a.ctas, 32 * WARPS, sm, st>>>(a, a.ctas);
   return (int)cudaGetLastError();
 }
 
 template <typename T, int HD>
 int launch_tc(const KvAttnArgs& a, cudaStream_t st) {
-  const size_t plan = (size_t)(a.B + 33) * 4;
-  if (a.rows == 16) {
-    const int mrows = std::min(16, a.T * a.group);
-    const size_t sm = FW * FS * few_stage<HD>() + (size_t)2 * mrows * (HD + 4 + 2) * 4;
-    return run_k(kv_attn_few_k<T, HD>, a, 32 * FW, std::max(sm, plan), st);
+  switch (a.rows) {
+    case 8: return run_tc<T, HD, 1, 1>(a, st);
+    case 16: return run_tc<T, HD, 2, 1>(a, st);
+    case 32: return run_tc<T, HD, 2, 2>(a, st);
+    default: return run_tc<T, HD, 2, 4>(a, st);
   }
-  constexpr int SB = 2 * rows_keys<HD>() * HD * 2;
-  if (a.rows == 32) return run_k(kv_attn_rows_k<T, HD, 2, 3>, a, 64, std::max<size_t>(3 * SB, plan), st);
-  if (a.rows == 64) return run_k(kv_attn_rows_k<T, HD, 4, 3>, a, 128, std::max<size_t>(3 * SB, plan), st);
-  return run_k(kv_attn_rows_k<T, HD, 8, 4>, a, 256, std::max<size_t>(4 * SB, plan), st);
 }
 
 }  // namespace kv
@@ -573,12 +487,14 @@ bool kv_attn_tc_takes(const KvAttnArgs& a, int dtype) {
 }
 
 void kv_attn_tc_plan(KvAttnArgs& a, int sms) {
-  const int R = a.T * a.group, few = a.hd > 64 ? s0::kv::few_keys<128>() : s0::kv::few_keys<64>();
-  a.rows = R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128;
+  using namespace s0::kv;
+  const int R = a.T * a.group;
+  a.rows = R <= 8 ? 8 : R <= 16 ? 16 : R <= 32 ? 32 : 64;
   a.nrb = (R + a.rows - 1) / a.rows;
-  a.tile = a.rows == 16 ? few : 64;
-  a.ctas = (a.rows == 128 ? 1 : 2) * sms;
-  a.min_per = a.rows == 16 ? 4 : 1;
+  const int wr = std::max(1, a.rows / 16);
+  a.tile = SLAB * wr / ((a.hd > 64 ? 128 : 64) * 4);
+  a.ctas = (wr == WARPS ? per_sm<WARPS>() : per_sm<1>()) * sms;
+  a.min_per = WARPS / wr;
   a.whole = 0;
 }
 

@@ -377,7 +377,9 @@ struct KvAttnArgs {
   // scratch: 2 * ctas pieces of [rows, hd] and [rows, 2]; with weights [B, nkv, T * group, sp] scores
   // and [B, nkv, T * group] log-sum-exps
   float *part_o, *part_ml, *scores, *lse;
+  int* prefix;                        // [B + 1] tiles of one (head, row block) before every sequence
   long sp;
+  float inv_group;                    // 1 / group
 };
 bool kv_attn_tc_takes(const KvAttnArgs& a, int dtype);
 void kv_attn_tc_plan(KvAttnArgs& a, int sms);
