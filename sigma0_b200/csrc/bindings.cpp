@@ -789,7 +789,7 @@ static void kv_caches(const at::Tensor& kc, const at::Tensor& vc, int64_t dim) {
   TORCH_CHECK(kc.dim() == dim && kc.sizes() == vc.sizes(), "the caches must have one shape [",
               dim == 5 ? "layers, " : "", "B, kv heads, slots, head dim]");
   TORCH_CHECK(kc.stride(-1) == 1 && vc.stride(-1) == 1, "the caches' head dimension must be contiguous");
-  TORCH_CHECK(kc.size(-2) < (int64_t)1 << 30 && kc.size(-1) >= 1, "cache too long");
+  TORCH_CHECK(kc.size(-1) >= 1 && kc.size(-2) * kc.size(-1) < (int64_t)1 << 31, "a head's slots x channels must stay below 2^31");
 }
 
 at::Tensor kv_attn(at::Tensor q, at::Tensor kn, at::Tensor vn, at::Tensor kc, at::Tensor vc, at::Tensor lengths,

@@ -315,17 +315,8 @@ int join(const KvAttnArgs& a, cudaStream_t st) {
   const long row_blocks = wide ? (rows + JT / 32 - 1) / (JT / 32) : rows;
   const long blocks = row_blocks + (a.weight ? (long)a.B * a.nkv * ((a.S + a.T + JW - 1) / JW) : 0);
   if (blocks == 0) return 0;                        // one CTA per unit and no weights: nothing is left to do
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)blocks);
-  cfg.blockDim = dim3(JT);
-  cfg.stream = st;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  return (int)(wide ? cudaLaunchKernelEx(&cfg, kv_join_k<T, 1>, a, (int)row_blocks)
-                    : cudaLaunchKernelEx(&cfg, kv_join_k<T, JT / 32>, a, (int)row_blocks));
+  return wide ? launch_after(kv_join_k<T, 1>, (unsigned)blocks, JT, st, a, (int)row_blocks)
+              : launch_after(kv_join_k<T, JT / 32>, (unsigned)blocks, JT, st, a, (int)row_blocks);
 }
 
 }  // namespace kv

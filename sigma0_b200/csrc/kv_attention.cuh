@@ -1,4 +1,4 @@
-// Shared parts of the cached-attention kernels (kv_attention.cu, kv_attention_tc.cu): how the
+// Shared parts of the cache kernels (kv_attention.cu, kv_attention_tc.cu, kv_evict.cu): how the
 // keys of all sequences are split over the CTAs, and element types.
 //
 // The lengths live on the device, so the host cannot balance a ragged batch.  Every CTA derives
@@ -170,9 +170,23 @@ S0_DEV long cta_share(Cur& c, const KvAttnArgs& a, int KT, int* scratch, int cta
   return min(p.total - w, p.per);
 }
 
-// Programmatic launch: the joining kernel may be set up while this one runs; it waits for its results.
+// Programmatic launch: the kernel behind this one may be set up while it runs, and waits for its results.
 S0_DEV void join_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 S0_DEV void join_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... P, typename... A>
+int launch_after(void (*k)(P...), unsigned blocks, int threads, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&cfg, k, P(args)...);
+}
 
 // base-2 log-sum-exp of a row; +inf where it saw nothing, so that exp2(s - lse) is 0 there
 S0_DEV float lse2(float m, float l) { return l == 0.f ? CUDART_INF_F : m + log2f(l); }

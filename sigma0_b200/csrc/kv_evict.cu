@@ -8,56 +8,128 @@
 // means nothing to the attention, so only what lies behind the new end moves: the i-th survivor
 // there goes to the i-th free slot before it.  That is at most len - keep rows, where closing the
 // gaps in order would move nearly all.
-//   evict_select_k   one block per unit: radix select of the threshold (four passes over 8 bits),
-//                    then ordered ranks by block scans; writes the metadata and the list of moves;
-//   evict_move_k     the rows of all units, 16 bytes a thread where the layout allows.
+// One block per unit: the keys go to shared memory (as far as they fit; beyond that they are formed
+// again on every pass), a radix select over 11 + 11 + 10 bits finds the threshold, block scans the ordered
+// ranks, and the block moves its own rows, so that the selection of some units runs under the traffic of
+// others.  What bounds it is that traffic: 8 bytes read and written per slot and the moved rows.  With
+// fewer units than SMs a second kernel moves the rows instead, with several blocks per unit.
 //
 // Acceptance.  The walk down a tree of drafted tokens takes the lowest child whose token is the
 // model's token after the node, until there is none; row len + path[j] moves to len + j.  A child
 // has a higher index than its parent, so path[j] >= j and rows can move upwards in order.
 #include <algorithm>
 
-#include "common.cuh"
-#include "launchers.h"
+#include "kv_attention.cuh"
 
 namespace s0 {
 namespace kv {
 
-constexpr int ET = 512;
+constexpr int EB = 2048;                 // bins of a pass of 11 bits
+constexpr uint32_t HELD = 0xffffffffu;   // stays whatever its weight
 
 S0_DEV uint32_t order_key(float w, int pos, int seen, const KvEvictArgs& a) {
-  if (pos >= seen - a.recent || pos < a.sinks) return 0xffffffffu;
+  if (pos >= seen - a.recent || pos < a.sinks) return HELD;
   if (w != w) return 0xfffffffeu;
   const uint32_t u = __float_as_uint(w + 0.f);  // -0 becomes 0
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// exclusive sums of three 0/1 flags of every thread (packed into 21 bits each) and their totals
-S0_DEV unsigned long long block_scan(unsigned long long v, unsigned long long* s_w, unsigned long long& total) {
+// exclusive sum over the block and the total; s_w: one value per warp and one more
+template <int NT, typename V>
+S0_DEV V block_scan(V v, V* s_w, V& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  unsigned long long inc = v;
+  V inc = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const unsigned long long y = __shfl_up_sync(0xffffffffu, inc, o);
+    const V y = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += y;
   }
   __syncthreads();
   if (lane == 31) s_w[warp] = inc;
   __syncthreads();
-  unsigned long long base = 0, sum = 0;
-  for (int w = 0; w < ET / 32; ++w) {
-    if (w < warp) base += s_w[w];
-    sum += s_w[w];
+  if (warp == 0) {
+    V x = lane < NT / 32 ? s_w[lane] : V(0), y = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const V z = __shfl_up_sync(0xffffffffu, y, o);
+      if (lane >= o) y += z;
+    }
+    if (lane < NT / 32) s_w[lane] = y - x;
+    if (lane == NT / 32 - 1) s_w[NT / 32] = y;
   }
-  total = sum;
-  return base + inc - v;
+  __syncthreads();
+  total = s_w[NT / 32];
+  return s_w[warp] + inc - v;
 }
 
-__global__ void __launch_bounds__(ET) evict_select_k(KvEvictArgs a) {
-  __shared__ int s_hist[256];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_need;
-  __shared__ unsigned long long s_w[ET / 32];
+// the rows of one unit's moves; V: the widest type that the rows' addresses and lengths are multiples of
+template <typename V>
+S0_DEV void move_rows(const KvEvictArgs& a, long u, int count, int i0, int step) {
+  const int h = (int)(u % a.nkv), b = (int)(u / a.nkv % a.B), n = (int)(u / a.nkv / a.B);
+  const unsigned C = a.hd * a.esize / (int)sizeof(V), total = count * C;
+  const int2* mv = a.moves + u * a.keep;
+  char* kc = (char*)a.kc + (n * a.kc_n + b * a.kc_b + h * a.kc_h) * a.esize;
+  char* vc = (char*)a.vc + (n * a.vc_n + b * a.vc_b + h * a.vc_h) * a.esize;
+  const long ks = a.kc_s * a.esize, vs = a.vc_s * a.esize;
+  constexpr int U = 4;                   // rows in flight per thread
+  for (unsigned i = i0; i < total; i += U * step) {
+    V k[U], v[U];
+    int to[U];
+#pragma unroll
+    for (int x = 0; x < U; ++x) {
+      const unsigned j = i + x * step;
+      if (j < total) {
+        const unsigned r = j / C;
+        const int2 m = mv[r];
+        const long c = (long)(j - r * C) * sizeof(V);
+        k[x] = *reinterpret_cast<const V*>(kc + m.x * ks + c);
+        v[x] = *reinterpret_cast<const V*>(vc + m.x * vs + c);
+        to[x] = m.y;
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < U; ++x) {
+      const unsigned j = i + x * step;
+      if (j < total) {
+        const long c = (long)(j % C) * sizeof(V);
+        *reinterpret_cast<V*>(kc + to[x] * ks + c) = k[x];
+        *reinterpret_cast<V*>(vc + to[x] * vs + c) = v[x];
+      }
+    }
+  }
+}
+S0_DEV void move_rows(const KvEvictArgs& a, long u, int count, int i0, int step) {
+  if (a.width == 16) move_rows<uint4>(a, u, count, i0, step);
+  else if (a.width == 8) move_rows<uint2>(a, u, count, i0, step);
+  else if (a.width == 4) move_rows<uint32_t>(a, u, count, i0, step);
+  else move_rows<uint16_t>(a, u, count, i0, step);
+}
+
+// The digit that holds the need-th largest value of a histogram: its bin, how many of it are needed.
+template <int NT>
+S0_DEV void find_digit(const int* hist, int need, int* s_w, int* s_found) {
+  constexpr int PER = EB / NT;
+  const int tid = threadIdx.x, top = EB - 1 - tid * PER;
+  int sum = 0, tot;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) sum += hist[top - k];
+  int above = block_scan<NT, int>(sum, s_w, tot);
+  if (above < need && need <= above + sum) {
+    int k = top;
+    while (above + hist[k] < need) above += hist[k--];
+    s_found[0] = k;
+    s_found[1] = need - above;
+    s_found[2] = hist[k];
+  }
+  __syncthreads();
+}
+
+template <int NT>
+__global__ void __launch_bounds__(NT) evict_k(KvEvictArgs a, int cached_keys, int moves_here) {
+  extern __shared__ __align__(16) uint32_t s_key[];    // [cached_keys]
+  __shared__ int s_hist[EB], s_w[NT / 32 + 1], s_found[3];
+  __shared__ unsigned long long s_w2[NT / 32 + 1];
+  join_may_start();
   const int tid = threadIdx.x;
   const long u = blockIdx.x;
   const int h = (int)(u % a.nkv), b = (int)(u / a.nkv % a.B), n = (int)(u / a.nkv / a.B);
@@ -67,89 +139,111 @@ __global__ void __launch_bounds__(ET) evict_select_k(KvEvictArgs a) {
   int* po = a.positions_out + n * a.po_n + b * a.po_b + h * a.po_h;
   const int len = min(max(a.lengths[b], 0), a.S), fin = min(len, a.keep), seen = a.seen[b];
   int2* mv = a.moves + u * a.keep;
+  const bool cut = len > fin, copy_w = wo != w, copy_p = po != p;
+  for (int i = tid; i < EB; i += NT) s_hist[i] = 0;
+  __syncthreads();
 
-  int moved = 0;
-  if (len > fin) {
-    // the fin-th largest key, 8 bits at a time; s_need: how many of the keys that share the prefix stay
-    if (tid == 0) { s_prefix = 0; s_need = fin; }
-    for (int sh = 24; sh >= 0; sh -= 8) {
-      if (tid < 256) s_hist[tid] = 0;
-      __syncthreads();
-      const uint32_t prefix = s_prefix, high = sh == 24 ? 0u : 0xffffffffu << (sh + 8);
-      for (int i = tid; i < len; i += ET) {
-        const uint32_t k = order_key(w[i], p[i], seen, a);
-        if ((k & high) == prefix) atomicAdd(&s_hist[(k >> sh) & 255], 1);
-      }
-      __syncthreads();
-      if (tid == 0) {
-        int need = s_need, d = 255;
-        while (d > 0 && s_hist[d] < need) need -= s_hist[d--];
-        s_prefix = prefix | ((uint32_t)d << sh);
-        s_need = need;
-      }
-      __syncthreads();
+  // keys, the first histogram, and what stays in place (free slots are overwritten later)
+  int held = 0;
+#pragma unroll 4
+  for (int i = tid; i < a.S; i += NT) {
+    const bool in = i < len;
+    const float x = in ? w[i] : 0.f;
+    const int y = in ? p[i] : -1;
+    if (cut && in) {
+      const uint32_t k = order_key(x, y, seen, a);
+      if (i < cached_keys) s_key[i] = k;
+      if (k == HELD) ++held;
+      else atomicAdd(&s_hist[k >> 21], 1);
     }
-    const uint32_t thr = s_prefix;
-    const int ties = s_need;
-    // ordered ranks: equal keys, free slots before the new end, survivors behind it
-    int eq0 = 0, hole0 = 0;
-    for (int i0 = 0; i0 < len; i0 += ET) {
-      const int i = i0 + tid;
-      const uint32_t k = i < len ? order_key(w[i], p[i], seen, a) : 0;
-      const bool in = i < len, eq = in && k == thr;
-      unsigned long long tot;
-      const int er = eq0 + (int)block_scan(eq, s_w, tot);
-      eq0 += (int)tot;
-      const bool stay = in && (k > thr || (eq && er < ties));
-      const bool hole = i < fin && !stay, mover = i >= fin && stay;
-      const unsigned long long at = block_scan((unsigned long long)hole | ((unsigned long long)mover << 32), s_w, tot);
-      if (hole) mv[hole0 + (int)(at & 0xffffffffu)].y = i;
-      if (mover) mv[moved + (int)(at >> 32)].x = i;
-      hole0 += (int)(tot & 0xffffffffu);
-      moved += (int)(tot >> 32);
+    if (copy_w) wo[i] = i < fin ? x : 0.f;
+    if (copy_p) po[i] = i < fin ? y : -1;
+  }
+  int moved = 0;
+  if (cut) {
+    auto key = [&](int i) { return i < cached_keys ? s_key[i] : order_key(w[i], p[i], seen, a); };
+    int all_held;
+    block_scan<NT, int>(held, s_w, all_held);
+    uint32_t thr = HELD;
+    int ties = fin, equal = all_held;
+    if (all_held < fin) {
+      find_digit<NT>(s_hist, fin - all_held, s_w, s_found);
+      uint32_t prefix = (uint32_t)s_found[0];
+      int need = s_found[1];
+#pragma unroll
+      for (int pass = 1; pass < 3; ++pass) {
+        const int sh = pass == 1 ? 10 : 0, bits = pass == 1 ? 11 : 10, above = sh + bits;
+        for (int i = tid; i < EB; i += NT) s_hist[i] = 0;
+        __syncthreads();
+        for (int i = tid; i < len; i += NT) {
+          const uint32_t k = key(i);
+          if (k >> above == prefix && k != HELD) atomicAdd(&s_hist[(k >> sh) & ((1u << bits) - 1)], 1);
+        }
+        __syncthreads();
+        find_digit<NT>(s_hist, need, s_w, s_found);
+        prefix = prefix << bits | (uint32_t)s_found[0];
+        need = s_found[1];
+      }
+      thr = prefix;
+      ties = need;
+      equal = s_found[2];
+    }
+    // Ordered ranks: every thread takes a run of slots (an odd number of them, so that the threads of a warp
+    // read different banks).  Equal keys first, if not all of them stay; then free slots before the new
+    // end and survivors behind it.
+    const int run = (len + NT - 1) / NT | 1, i0 = min(len, tid * run), i1 = min(len, i0 + run);
+    int rank = 0;
+    if (equal != ties) {
+      int e = 0, tot;
+      for (int i = i0; i < i1; ++i) e += key(i) == thr;
+      rank = block_scan<NT, int>(e, s_w, tot);
+    }
+    const int rank0 = rank;
+    unsigned long long mine = 0, tot2;
+    for (int i = i0; i < i1; ++i) {
+      const uint32_t k = key(i);
+      const bool stay = k > thr || (k == thr && rank++ < ties);
+      if (i < fin) mine += !stay;
+      else mine += (unsigned long long)stay << 32;
+    }
+    const unsigned long long at = block_scan<NT, unsigned long long>(mine, s_w2, tot2);
+    int hole = (int)(at & 0xffffffffu), mover = (int)(at >> 32);
+    moved = (int)(tot2 >> 32);
+    rank = rank0;
+    for (int i = i0; i < i1; ++i) {
+      const uint32_t k = key(i);
+      const bool stay = k > thr || (k == thr && rank++ < ties);
+      if (i < fin && !stay) mv[hole++].y = i;
+      if (i >= fin && stay) mv[mover++].x = i;
     }
   }
   if (tid == 0) a.count[u] = moved;
-  // metadata: what stays in place, then the moved, then the free slots (read before they are cleared
-  // when the outputs are the inputs)
-  if (wo != w)
-    for (int i = tid; i < fin; i += ET) wo[i] = w[i];
-  if (po != p)
-    for (int i = tid; i < fin; i += ET) po[i] = p[i];
   __syncthreads();
-  for (int j = tid; j < moved; j += ET) {
+  for (int j = tid; j < moved; j += NT) {
     const int2 m = mv[j];
     wo[m.y] = w[m.x];
     po[m.y] = p[m.x];
   }
-  __syncthreads();
-  for (int i = fin + tid; i < a.S; i += ET) {
-    wo[i] = 0.f;
-    po[i] = -1;
+  if (!copy_w || !copy_p) {
+    __syncthreads();                       // the survivors have been read
+    for (int i = fin + tid; i < a.S; i += NT) {
+      if (!copy_w) wo[i] = 0.f;
+      if (!copy_p) po[i] = -1;
+    }
   }
+  if (!moves_here) return;
+  if (a.lengths_out != a.lengths && u < (long)a.B * a.nkv && h == 0 && tid == 0) a.lengths_out[b] = fin;
+  move_rows(a, u, moved, tid, NT);
 }
 
-// V: the widest type that the rows' addresses and lengths are multiples of
-template <typename V>
+// the rows of all units, `parts` blocks each, and the new lengths; parts 0: the lengths only
 __global__ void __launch_bounds__(256) evict_move_k(KvEvictArgs a, int parts) {
+  join_wait();
+  if (blockIdx.x == 0)
+    for (int b = threadIdx.x; b < a.B; b += 256) a.lengths_out[b] = min(min(max(a.lengths[b], 0), a.S), a.keep);
+  if (parts == 0) return;
   const long u = blockIdx.x / parts;
-  const int part = (int)(blockIdx.x % parts);
-  const int h = (int)(u % a.nkv), b = (int)(u / a.nkv % a.B), n = (int)(u / a.nkv / a.B);
-  const int C = a.hd * a.esize / (int)sizeof(V);
-  const long count = a.count[u];
-  const int2* mv = a.moves + u * a.keep;
-  char* kc = (char*)a.kc + (n * a.kc_n + b * a.kc_b + h * a.kc_h) * a.esize;
-  char* vc = (char*)a.vc + (n * a.vc_n + b * a.vc_b + h * a.vc_h) * a.esize;
-  const long ks = a.kc_s * a.esize, vs = a.vc_s * a.esize;
-  for (long i = (long)part * 256 + threadIdx.x; i < count * C; i += 256L * parts) {
-    const int2 m = mv[i / C];
-    const long c = i % C * (long)sizeof(V);
-    const V k = *reinterpret_cast<const V*>(kc + m.x * ks + c), v = *reinterpret_cast<const V*>(vc + m.x * vs + c);
-    *reinterpret_cast<V*>(kc + m.y * ks + c) = k;
-    *reinterpret_cast<V*>(vc + m.y * vs + c) = v;
-  }
-  if (u < (long)a.B * a.nkv && h == 0 && part == 0 && threadIdx.x == 0)
-    a.lengths_out[b] = min(min(max(a.lengths[b], 0), a.S), a.keep);
+  move_rows(a, u, a.count[u], (int)(blockIdx.x % parts) * 256 + threadIdx.x, 256 * parts);
 }
 
 constexpr int CT = 512, CMAX = 1024;
@@ -249,21 +343,28 @@ int width_of(int hd, int es, std::initializer_list<long> strides, std::initializ
 }  // namespace kv
 }  // namespace s0
 
-int kv_evict_launch(const KvEvictArgs& a, cudaStream_t st) {
+template <int NT>
+static int select_units(const KvEvictArgs& a, unsigned units, int keys, int moves_here, cudaStream_t st) {
+  const cudaError_t e = cudaFuncSetAttribute(s0::kv::evict_k<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, keys * 4);
+  if (e != cudaSuccess) return (int)e;
+  s0::kv::evict_k<NT><<<units, NT, (size_t)keys * 4, st>>>(a, keys, moves_here);
+  return (int)cudaGetLastError();
+}
+
+int kv_evict_launch(KvEvictArgs a, cudaStream_t st) {
   using namespace s0::kv;
   const long units = (long)a.N * a.B * a.nkv;
   if (units <= 0) return 0;
-  evict_select_k<<<(unsigned)units, ET, 0, st>>>(a);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return (int)e;
-  const int v = width_of(a.hd, a.esize, {a.kc_n, a.kc_b, a.kc_h, a.kc_s, a.vc_n, a.vc_b, a.vc_h, a.vc_s}, {a.kc, a.vc});
-  const int parts = (int)std::max<long>(1, std::min<long>(16, (8L * a.sms + units - 1) / units));
-  const unsigned grid = (unsigned)(units * parts);
-  if (v == 16) evict_move_k<uint4><<<grid, 256, 0, st>>>(a, parts);
-  else if (v == 8) evict_move_k<uint2><<<grid, 256, 0, st>>>(a, parts);
-  else if (v == 4) evict_move_k<uint32_t><<<grid, 256, 0, st>>>(a, parts);
-  else evict_move_k<uint16_t><<<grid, 256, 0, st>>>(a, parts);
-  return (int)cudaGetLastError();
+  a.width = width_of(a.hd, a.esize, {a.kc_n, a.kc_b, a.kc_h, a.kc_s, a.vc_n, a.vc_b, a.vc_h, a.vc_s}, {a.kc, a.vc});
+  const bool here = units >= a.sms;                        // enough units to keep the memory busy by themselves
+  const int keys = std::min(a.S, 50 * 1024);               // 200 KB of keys at most
+  // few long units: more threads shorten the passes over the keys
+  const int rc = !here && a.S > 2048 ? select_units<1024>(a, (unsigned)units, keys, here, st)
+                                     : select_units<256>(a, (unsigned)units, keys, here, st);
+  if (rc || (here && a.lengths_out != a.lengths)) return rc;
+  // lengths that are overwritten in place wait for all units to have read them
+  const int parts = here ? 0 : (int)std::max<long>(1, std::min<long>(32, (8L * a.sms + units - 1) / units));
+  return launch_after(evict_move_k, parts ? (unsigned)(units * parts) : 1u, 256, st, a, parts);
 }
 
 int kv_commit_launch(const KvCommitArgs& a, cudaStream_t st) {

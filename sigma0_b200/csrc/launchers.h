@@ -400,11 +400,12 @@ struct KvEvictArgs {
   long w_n, w_b, w_h, p_n, p_b, p_h, wo_n, wo_b, wo_h, po_n, po_b, po_h;
   int N, B, nkv, S, hd, esize;
   int keep, recent, sinks;
+  int width;                          // set by the launcher: bytes of the widest aligned access
   int2* moves;                        // scratch [N * B * nkv, keep]: (from, to) slots
   int* count;                         // scratch [N * B * nkv]
   int sms;
 };
-int kv_evict_launch(const KvEvictArgs& a, cudaStream_t st);
+int kv_evict_launch(KvEvictArgs a, cudaStream_t st);
 
 // acceptance of a drafted tree (kv_evict.cu)
 struct KvCommitArgs {
