@@ -64,14 +64,13 @@ S0_DEV V block_scan(V v, V* s_w, V& total) {
 
 // the rows of one unit's moves; V: the widest type that the rows' addresses and lengths are multiples of
 template <typename V>
-S0_DEV void move_rows(const KvEvictArgs& a, long u, int count, int i0, int step) {
+S0_DEV void move_rows(const KvEvictArgs& a, const int2* mv, long u, int count, int i0, int step) {
   const int h = (int)(u % a.nkv), b = (int)(u / a.nkv % a.B), n = (int)(u / a.nkv / a.B);
   const unsigned C = a.hd * a.esize / (int)sizeof(V), total = count * C;
-  const int2* mv = a.moves + u * a.keep;
   char* kc = (char*)a.kc + (n * a.kc_n + b * a.kc_b + h * a.kc_h) * a.esize;
   char* vc = (char*)a.vc + (n * a.vc_n + b * a.vc_b + h * a.vc_h) * a.esize;
   const long ks = a.kc_s * a.esize, vs = a.vc_s * a.esize;
-  constexpr int U = 4;                   // rows in flight per thread
+  constexpr int U = 2;                   // pairs of rows in flight per thread
   for (unsigned i = i0; i < total; i += U * step) {
     V k[U], v[U];
     int to[U];
@@ -98,11 +97,11 @@ S0_DEV void move_rows(const KvEvictArgs& a, long u, int count, int i0, int step)
     }
   }
 }
-S0_DEV void move_rows(const KvEvictArgs& a, long u, int count, int i0, int step) {
-  if (a.width == 16) move_rows<uint4>(a, u, count, i0, step);
-  else if (a.width == 8) move_rows<uint2>(a, u, count, i0, step);
-  else if (a.width == 4) move_rows<uint32_t>(a, u, count, i0, step);
-  else move_rows<uint16_t>(a, u, count, i0, step);
+S0_DEV void move_rows(const KvEvictArgs& a, const int2* mv, long u, int count, int i0, int step) {
+  if (a.width == 16) move_rows<uint4>(a, mv, u, count, i0, step);
+  else if (a.width == 8) move_rows<uint2>(a, mv, u, count, i0, step);
+  else if (a.width == 4) move_rows<uint32_t>(a, mv, u, count, i0, step);
+  else move_rows<uint16_t>(a, mv, u, count, i0, step);
 }
 
 // The digit that holds the need-th largest value of a histogram: its bin, how many of it are needed.
@@ -124,9 +123,10 @@ S0_DEV void find_digit(const int* hist, int need, int* s_w, int* s_found) {
   __syncthreads();
 }
 
-template <int NT>
-__global__ void __launch_bounds__(NT) evict_k(KvEvictArgs a, int cached_keys, int moves_here) {
-  extern __shared__ __align__(16) uint32_t s_key[];    // [cached_keys]
+// KEYS: all keys fit into shared memory
+template <int NT, bool KEYS>
+__global__ void __launch_bounds__(NT, 1536 / NT) evict_k(KvEvictArgs a, int moves_here) {
+  extern __shared__ __align__(16) uint32_t s_key[];    // [S], later the list of moves
   __shared__ int s_hist[EB], s_w[NT / 32 + 1], s_found[3];
   __shared__ unsigned long long s_w2[NT / 32 + 1];
   join_may_start();
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(NT) evict_k(KvEvictArgs a, int cached_keys, in
     const int y = in ? p[i] : -1;
     if (cut && in) {
       const uint32_t k = order_key(x, y, seen, a);
-      if (i < cached_keys) s_key[i] = k;
+      if (KEYS) s_key[i] = k;
       if (k == HELD) ++held;
       else atomicAdd(&s_hist[k >> 21], 1);
     }
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(NT) evict_k(KvEvictArgs a, int cached_keys, in
   }
   int moved = 0;
   if (cut) {
-    auto key = [&](int i) { return i < cached_keys ? s_key[i] : order_key(w[i], p[i], seen, a); };
+    auto key = [&](int i) { return KEYS ? s_key[i] : order_key(w[i], p[i], seen, a); };
     int all_held;
     block_scan<NT, int>(held, s_w, all_held);
     uint32_t thr = HELD;
@@ -198,34 +198,43 @@ __global__ void __launch_bounds__(NT) evict_k(KvEvictArgs a, int cached_keys, in
       for (int i = i0; i < i1; ++i) e += key(i) == thr;
       rank = block_scan<NT, int>(e, s_w, tot);
     }
+    // 64 slots of a run at a time: which of them are free, which move
+    auto flags = [&](int s0, unsigned long long& holes, unsigned long long& movers) {
+      holes = movers = 0;
+      for (int i = s0; i < min(i1, s0 + 64); ++i) {
+        const uint32_t k = key(i);
+        const bool stay = k > thr || (k == thr && rank++ < ties);
+        if (i < fin && !stay) holes |= 1ull << (i - s0);
+        if (i >= fin && stay) movers |= 1ull << (i - s0);
+      }
+    };
     const int rank0 = rank;
-    unsigned long long mine = 0, tot2;
-    for (int i = i0; i < i1; ++i) {
-      const uint32_t k = key(i);
-      const bool stay = k > thr || (k == thr && rank++ < ties);
-      if (i < fin) mine += !stay;
-      else mine += (unsigned long long)stay << 32;
+    unsigned long long holes = 0, movers = 0, mine = 0, tot2;
+    for (int s0 = i0; s0 < i1; s0 += 64) {
+      flags(s0, holes, movers);
+      mine += (unsigned long long)__popcll(holes) | (unsigned long long)__popcll(movers) << 32;
     }
     const unsigned long long at = block_scan<NT, unsigned long long>(mine, s_w2, tot2);
     int hole = (int)(at & 0xffffffffu), mover = (int)(at >> 32);
     moved = (int)(tot2 >> 32);
     rank = rank0;
-    for (int i = i0; i < i1; ++i) {
-      const uint32_t k = key(i);
-      const bool stay = k > thr || (k == thr && rank++ < ties);
-      if (i < fin && !stay) mv[hole++].y = i;
-      if (i >= fin && stay) mv[mover++].x = i;
+    for (int s0 = i0; s0 < i1; s0 += 64) {
+      if (i1 - i0 > 64) flags(s0, holes, movers);
+      for (; holes; holes &= holes - 1) mv[hole++].y = s0 + __ffsll(holes) - 1;
+      for (; movers; movers &= movers - 1) mv[mover++].x = s0 + __ffsll(movers) - 1;
     }
   }
   if (tid == 0) a.count[u] = moved;
   __syncthreads();
+  int2* list = KEYS ? reinterpret_cast<int2*>(s_key) : mv;  // a move takes one of two slots: it fits
   for (int j = tid; j < moved; j += NT) {
     const int2 m = mv[j];
+    if (KEYS) list[j] = m;
     wo[m.y] = w[m.x];
     po[m.y] = p[m.x];
   }
-  if (!copy_w || !copy_p) {
-    __syncthreads();                       // the survivors have been read
+  __syncthreads();
+  if (!copy_w || !copy_p) {                // the survivors have been read
     for (int i = fin + tid; i < a.S; i += NT) {
       if (!copy_w) wo[i] = 0.f;
       if (!copy_p) po[i] = -1;
@@ -233,7 +242,7 @@ __global__ void __launch_bounds__(NT) evict_k(KvEvictArgs a, int cached_keys, in
   }
   if (!moves_here) return;
   if (a.lengths_out != a.lengths && u < (long)a.B * a.nkv && h == 0 && tid == 0) a.lengths_out[b] = fin;
-  move_rows(a, u, moved, tid, NT);
+  move_rows(a, list, u, moved, tid, NT);
 }
 
 // the rows of all units, `parts` blocks each, and the new lengths; parts 0: the lengths only
@@ -243,7 +252,7 @@ __global__ void __launch_bounds__(256) evict_move_k(KvEvictArgs a, int parts) {
     for (int b = threadIdx.x; b < a.B; b += 256) a.lengths_out[b] = min(min(max(a.lengths[b], 0), a.S), a.keep);
   if (parts == 0) return;
   const long u = blockIdx.x / parts;
-  move_rows(a, u, a.count[u], (int)(blockIdx.x % parts) * 256 + threadIdx.x, 256 * parts);
+  move_rows(a, a.moves + u * a.keep, u, a.count[u], (int)(blockIdx.x % parts) * 256 + threadIdx.x, 256 * parts);
 }
 
 constexpr int CT = 512, CMAX = 1024;
@@ -343,11 +352,12 @@ int width_of(int hd, int es, std::initializer_list<long> strides, std::initializ
 }  // namespace kv
 }  // namespace s0
 
-template <int NT>
-static int select_units(const KvEvictArgs& a, unsigned units, int keys, int moves_here, cudaStream_t st) {
-  const cudaError_t e = cudaFuncSetAttribute(s0::kv::evict_k<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, keys * 4);
+template <int NT, bool KEYS>
+static int select_units(const KvEvictArgs& a, unsigned units, int moves_here, cudaStream_t st) {
+  const size_t sm = KEYS ? (size_t)a.S * 4 + 8 : 0;
+  const cudaError_t e = cudaFuncSetAttribute(s0::kv::evict_k<NT, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
   if (e != cudaSuccess) return (int)e;
-  s0::kv::evict_k<NT><<<units, NT, (size_t)keys * 4, st>>>(a, keys, moves_here);
+  s0::kv::evict_k<NT, KEYS><<<units, NT, sm, st>>>(a, moves_here);
   return (int)cudaGetLastError();
 }
 
@@ -357,10 +367,13 @@ int kv_evict_launch(KvEvictArgs a, cudaStream_t st) {
   if (units <= 0) return 0;
   a.width = width_of(a.hd, a.esize, {a.kc_n, a.kc_b, a.kc_h, a.kc_s, a.vc_n, a.vc_b, a.vc_h, a.vc_s}, {a.kc, a.vc});
   const bool here = units >= a.sms;                        // enough units to keep the memory busy by themselves
-  const int keys = std::min(a.S, 50 * 1024);               // 200 KB of keys at most
-  // few long units: more threads shorten the passes over the keys
-  const int rc = !here && a.S > 2048 ? select_units<1024>(a, (unsigned)units, keys, here, st)
-                                     : select_units<256>(a, (unsigned)units, keys, here, st);
+  // Threads per unit: keys of more than 24 KB leave no more than six blocks on an SM whatever their size, so
+  // those are larger; few units on an otherwise empty GPU take still more.  200 KB of keys at most.
+  const bool fits = a.S <= 50 * 1024;
+  const unsigned n = (unsigned)units;
+  const int rc = !fits ? select_units<512, false>(a, n, here, st)
+                 : a.S <= 6 * 1024 && (here || a.S <= 2048) ? select_units<256, true>(a, n, here, st)
+                 : here ? select_units<512, true>(a, n, here, st) : select_units<1024, true>(a, n, here, st);
   if (rc || (here && a.lengths_out != a.lengths)) return rc;
   // lengths that are overwritten in place wait for all units to have read them
   const int parts = here ? 0 : (int)std::max<long>(1, std::min<long>(32, (8L * a.sms + units - 1) / units));
