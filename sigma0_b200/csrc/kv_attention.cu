@@ -1,5 +1,5 @@
-// Attention of a few new tokens over a key / value cache: the kernel for any element type, head
-// size and alignment, and the kernel that joins the pieces of a split (kv_attention_tc.cu has the
+// Attention of a few new tokens over a key / value cache: the fp32 kernel for any element
+// type, head size up to 512 and alignment, and the kernel that joins the pieces of a split (kv_attention_tc.cu has the
 // tensor-core kernel for aligned 16-bit caches).
 //
 // Row r = (new token t, query head g of the key head's group) attends to the len cached keys and
@@ -16,163 +16,350 @@
 namespace s0 {
 namespace kv {
 
-constexpr int GT = 128;  // threads of the general kernel
-constexpr int GK = 32;   // keys of a tile: one per lane in the softmax
-constexpr int GR = 8;    // query rows of a block: two per warp
-constexpr int GC = 4;    // output columns of a thread: heads up to GT * GC wide
+constexpr int SW = 4;  // warps of a block
 
-// The general kernel: everything in fp32, one K (then V) tile in shared memory at a time; element
-// loads, so any stride and alignment will do.
-template <typename T>
-__global__ void __launch_bounds__(GT) kv_attn_any_k(KvAttnArgs a) {
-  extern __shared__ __align__(16) unsigned char smem[];
-  const int hd = a.hd, ldk = hd | 1;           // odd row stride: lanes read 32 rows at one column
-  float* sQ = reinterpret_cast<float*>(smem);  // [GR][hd]
-  float* sT = sQ + GR * hd;                    // [GK][ldk]
-  float* sP = sT + GK * ldk;                   // [GR][GK]
-  float* sA = sP + GR * GK;                    // [GR] rescale, then 1 / sum
-  uint32_t* sV = reinterpret_cast<uint32_t*>(sA + GR);  // [GR] visible keys of the tile
-  int* s_pre = reinterpret_cast<int*>(sV + GR);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int R = a.T * a.group;
+// Keys of a slab: one per lane (64 channels), or per 2 or 4 lanes that share its channels.  Its rows lie
+// lane_parts * 4 words apart modulo 32 banks, so that the 8 lanes of a 16-byte access hit different banks.
+template <int HDP> constexpr int lane_parts() { return HDP == 64 ? 1 : HDP == 128 ? 2 : 4; }
+template <int HDP> constexpr int slab_keys() { return 32 / lane_parts<HDP>(); }
+template <int HDP> constexpr int slab_ld() { return HDP + 4 * lane_parts<HDP>(); }
+template <int HDP> constexpr int most_rows() { return HDP == 64 ? 32 : HDP == 128 ? 16 : 8; }
+template <int HDP, int RB> constexpr size_t simt_bytes() {
+  return 4 * ((size_t)SW * 2 * slab_keys<HDP>() * slab_ld<HDP>()   // K and V slabs
+              + RB * HDP                                          // queries
+              + SW * RB * (slab_keys<HDP>() + 4)                   // probabilities
+              + 2 * RB * (HDP + 2));                               // two warps' results
+}
+
+// HDP: the head size padded to 64, 128, 256 or 512; RB: rows of a block; a.vec: 16-byte rows of floats.
+//
+// Every warp streams slabs of keys of its own (kv_attention_tc.cu does the same).  Scores: a lane holds
+// its key's channels in registers and reads the queries as broadcasts, 4 products per 16-byte load of
+// shared memory and row.  Output: a lane owns HDP / 32 channels of all rows, reads V once and the
+// probabilities as broadcasts.  K of the next slab is fetched while V is used and the other way round.
+// What bounds it: HBM for few rows (4 bytes per channel), the fp32 pipe from some 16 rows on.
+template <typename T, int HDP, int RB>
+__global__ void __launch_bounds__(32 * SW, HDP == 512 ? 1 : 2) kv_attn_any_k(KvAttnArgs a, int ctas) {
+  constexpr int DL = lane_parts<HDP>(), NK = slab_keys<HDP>(), LD = slab_ld<HDP>(), PL = NK + 4;
+  constexpr int COLS = HDP / 32, RG = RB < 4 ? RB : 4;             // channels of a lane; rows at a time in the scores
+  constexpr int KQ = HDP / DL / 4, KH = KQ < 16 ? KQ : 16;         // 16-byte groups of a lane, of them in registers
+  constexpr int JS = COLS > 8 ? 2 : 4;                             // keys at a time in the output
+  extern __shared__ __align__(16) float s_f[];
   join_may_start();
-  const Plan plan = make_plan(a, plan_prefix(a, GK, s_pre), gridDim.x, a.min_per);
-  if (blockIdx.x == 0)
-    for (int i = tid; i <= a.B; i += GT) a.prefix[i] = s_pre[i];
-  long w = blockIdx.x * plan.per;
-  const long wend = min(plan.total, w + plan.per);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kl = lane / DL, dl = lane % DL;
+  const int R = a.T * a.group;
+  float* sK = s_f + warp * 2 * NK * LD;
+  float* sV = sK + NK * LD;
+  float* sQ = s_f + SW * 2 * NK * LD;                              // [RB][HDP], scaled
+  float* sP = sQ + RB * HDP + warp * RB * PL;                      // [RB][PL]
+  float* sJ = sQ + RB * HDP + SW * RB * PL;                        // [2][RB][HDP]
+  float* sM = sJ + 2 * RB * HDP;                                   // [2][RB][2]
+  Cur cur;
+  const long share = cta_share(cur, a, NK, reinterpret_cast<int*>(s_f), ctas);
+  __syncthreads();
+  if (share <= 0) return;
+  for (int i = tid; i < SW * 2 * NK * LD; i += 32 * SW) s_f[i] = 0.f;   // channels past hd stay 0
+  __syncthreads();
 
-  while (w < wend) {
-    const Seg sg = find_seg(a, s_pre, w, GK);
-    const int t1 = (int)min((long)sg.n, sg.t0 + (wend - w));
-    const int b = sg.b, h = sg.h, r0 = sg.rb * GR, nr = min(GR, R - r0);
-    const int ncache = (sg.len + GK - 1) / GK;
-    T* kc = (T*)a.kc + b * a.kc_b + h * a.kc_h;
-    T* vc = (T*)a.vc + b * a.vc_b + h * a.vc_h;
-    const T* kn = (const T*)a.kn + b * a.kn_b + h * a.kn_h;
-    const T* vn = (const T*)a.vn + b * a.vn_b + h * a.vn_h;
-    for (int i = tid; i < GR * hd; i += GT) {
-      const int r = i / hd, d = i - r * hd;
-      float x = 0.f;
-      if (r < nr) {
-        const int row = r0 + r, t = row / a.group, g = row - t * a.group;
-        x = Elem<T>::to(((const T*)a.q)[b * a.q_b + t * a.q_t + (h * a.group + g) * a.q_h + d]) * a.scale_log2;
-      }
-      sQ[i] = x;
-    }
-    float acc[GC][GR];
+  Cur ahead = cur;
+  int left = (int)((share - warp + SW - 1) / SW);
+  if (left > 0) cur_skip(ahead, a, NK, warp);
+  // rows of K (then V) of the next slab; a row that does not exist becomes 0
+  auto fetch = [&](float* dst, bool value) {
+    if (left > 0) {
+      const int ncache = (ahead.len + NK - 1) / NK, h = ahead.u / a.nrb;
+      const bool tail = ahead.t >= ncache;
+      const int k0 = (tail ? ahead.t - ncache : ahead.t) * NK, rows = (tail ? a.T : ahead.len) - k0;
+      const long rs = value ? (tail ? a.vn_t : a.vc_s) : (tail ? a.kn_t : a.kc_s);
+      const T* src = (value ? (tail ? (const T*)a.vn + ahead.b * a.vn_b + h * a.vn_h : (const T*)a.vc + ahead.b * a.vc_b + h * a.vc_h)
+                            : (tail ? (const T*)a.kn + ahead.b * a.kn_b + h * a.kn_h : (const T*)a.kc + ahead.b * a.kc_b + h * a.kc_h)) +
+                     (long)k0 * rs;
+      if constexpr (sizeof(T) == 4) {
+        if (a.vec) {
+          constexpr int C = HDP / 4, L = C < 32 ? C : 32;          // groups of a row, lanes on a row
 #pragma unroll
-    for (int c = 0; c < GC; ++c)
+          for (int r = lane / L; r < NK; r += 32 / L)
 #pragma unroll
-      for (int r = 0; r < GR; ++r) acc[c][r] = 0.f;
-    float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};  // rows 2 warp, 2 warp + 1
-
-    for (int tt = sg.t0; tt < t1; ++tt) {
-      const bool tail = tt >= ncache;
-      const int k0 = (tail ? tt - ncache : tt) * GK, lim = tail ? a.T : sg.len;
-      const int nk = min(GK, lim - k0);
-      const bool put = tail && sg.rb == 0;
-      auto load = [&](T* cache, long cs, const T* fresh, long fs) {
-        for (int i = tid; i < GK * hd; i += GT) {
-          const int j = i / hd, d = i - j * hd;
-          T x = Elem<T>::of(0.f);                       // a key past the end contributes 0 * 0
-          if (j < nk) {
-            x = tail ? fresh[(k0 + j) * fs + d] : cache[(k0 + j) * cs + d];
-            if (put && sg.len + k0 + j < a.S) cache[(long)(sg.len + k0 + j) * cs + d] = x;
-          }
-          sT[j * ldk + d] = Elem<T>::to(x);
-        }
-      };
-      __syncthreads();
-      load(kc, a.kc_s, kn, a.kn_t);
-      __syncthreads();
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int r = 2 * warp + q, row = r0 + r;
-        float s0 = 0.f, s1 = 0.f;
-        const float *qr = sQ + r * hd, *kr = sT + lane * ldk;
-        int d = 0;
-        for (; d + 1 < hd; d += 2) {
-          s0 = fmaf(qr[d], kr[d], s0);
-          s1 = fmaf(qr[d + 1], kr[d + 1], s1);
-        }
-        if (d < hd) s0 = fmaf(qr[d], kr[d], s0);
-        float s = s0 + s1;
-        const bool vis = lane < nk && r < nr && (!tail || sees(a, b, row / a.group, k0 + lane));
-        if (!vis) s = -CUDART_INF_F;
-        const uint32_t seen = __ballot_sync(0xffffffffu, vis);
-        if (a.scores && lane < nk && r < nr)
-          a.scores[(((long)b * a.nkv + h) * R + row) * a.sp + (tail ? sg.len : 0) + k0 + lane] = s;
-        float mx = s;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        mx = fmaxf(mx, m[q]);
-        const float base = mx == -CUDART_INF_F ? 0.f : mx;
-        const float al = exp2f(m[q] - base), p = exp2f(s - base);
-        m[q] = mx;
-        l[q] = l[q] * al + warp_sum(p);
-        sP[r * GK + lane] = p;
-        if (lane == 0) {
-          sA[r] = al;
-          sV[r] = seen;
-        }
-      }
-      __syncthreads();
-      load(vc, a.vc_s, vn, a.vn_t);
-      __syncthreads();
-#pragma unroll
-      for (int r = 0; r < GR; ++r) {
-        const float al = sA[r];
-#pragma unroll
-        for (int c = 0; c < GC; ++c) acc[c][r] *= al;
-      }
-      for (int j = 0; j < nk; ++j) {
-        float v[GC];
-#pragma unroll
-        for (int c = 0; c < GC; ++c) v[c] = tid + c * GT < hd ? sT[j * ldk + tid + c * GT] : 0.f;
-#pragma unroll
-        for (int r = 0; r < GR; ++r) {
-          const float p = sP[r * GK + j];
-#pragma unroll
-          for (int c = 0; c < GC; ++c)
-            if (!tail || (sV[r] >> j & 1)) acc[c][r] = fmaf(p, v[c], acc[c][r]);  // 0 times a hidden infinity stays out
-        }
-      }
-      if (put && a.positions && tid < nk && sg.len + k0 + tid < a.S)
-        a.positions[b * a.pos_b + h * a.pos_h + sg.len + k0 + tid] = a.seen[b] + k0 + tid;
-    }
-
-    const bool first = sg.t0 == 0, last = t1 == sg.n;
-    const long slot = 2L * blockIdx.x + (first ? 1 : 0);
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int r = 2 * warp + q;
-      if (lane == 0) {
-        if (first && last) {
-          sA[r] = l[q] == 0.f ? 0.f : 1.f / l[q];
-          if (a.lse && r < nr) a.lse[((long)b * a.nkv + h) * R + r0 + r] = lse2(m[q], l[q]);
+            for (int c = lane % L; c < C; c += L)
+              if (c * 4 < a.hd) cp_async16(dst + r * LD + c * 4, r < rows ? src + r * rs + c * 4 : src, r < rows ? 16 : 0);
         } else {
-          a.part_ml[(slot * a.rows + r) * 2] = m[q];
-          a.part_ml[(slot * a.rows + r) * 2 + 1] = l[q];
+          for (int r = 0; r < NK; ++r)
+            for (int d = lane; d < a.hd; d += 32) cp_async4(dst + r * LD + d, r < rows ? src + r * rs + d : src, r < rows ? 4 : 0);
+        }
+      } else {
+        constexpr int U = 4;                                       // loads in flight per lane
+        for (int r = 0; r < NK; ++r)
+          for (int d0 = lane; d0 < a.hd; d0 += 32 * U) {
+            T x[U];
+#pragma unroll
+            for (int k = 0; k < U; ++k) x[k] = r < rows && d0 + 32 * k < a.hd ? src[r * rs + d0 + 32 * k] : Elem<T>::of(0.f);
+#pragma unroll
+            for (int k = 0; k < U; ++k)
+              if (d0 + 32 * k < a.hd) dst[r * LD + d0 + 32 * k] = Elem<T>::to(x[k]);
+          }
+      }
+      if (value && --left > 0) cur_skip(ahead, a, NK, SW);
+    }
+    cp_async_commit();
+  };
+  fetch(sK, false);
+  fetch(sV, true);
+
+  long done = 0, mine = warp;
+  while (done < share) {
+    const int b = cur.b, h = cur.u / a.nrb, rb = cur.u - h * a.nrb, r0 = rb * RB, nr = min(RB, R - r0);
+    const long bh = (long)b * a.nkv + h;
+    const int t1 = (int)min((long)cur.n, cur.t + (share - done));
+    const int ncache = (cur.len + NK - 1) / NK;
+    const long end = done + (t1 - cur.t);
+    __syncthreads();                                               // the last unit's queries have been read
+    for (int i = tid; i < RB * HDP; i += 32 * SW) {
+      const int r = i / HDP, d = i % HDP, tok = div_group(a, r0 + r);
+      sQ[i] = r < nr && d < a.hd ? Elem<T>::to(((const T*)a.q)[b * a.q_b + tok * a.q_t + (long)(h * a.group + r0 + r - tok * a.group) * a.q_h + d]) * a.scale_log2
+                                 : 0.f;
+    }
+    __syncthreads();
+    float o[RB][COLS];
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int c = 0; c < COLS; ++c) o[r][c] = 0.f;
+    float m = -CUDART_INF_F, l = 0.f;                              // of row `lane`
+
+    for (; mine < end; mine += SW) {
+      const int tt = cur.t + (int)(mine - done);
+      const bool tail = tt >= ncache;
+      const int k0 = (tail ? tt - ncache : tt) * NK, nk = min(NK, (tail ? a.T : cur.len) - k0);
+      cp_async_wait_group<1>();
+      __syncwarp();
+      // ---- scores, row group by row group --------------------------------------------------------
+      float al = 1.f;                                              // rescaling of row `lane`
+      bool moved = false;
+#pragma unroll 1
+      for (int rg = 0; rg < nr; rg += RG) {
+        float s[RG];
+#pragma unroll
+        for (int r = 0; r < RG; ++r) s[r] = 0.f;
+#pragma unroll
+        for (int half = 0; half < KQ / KH; ++half) {
+          float4 k[KH];
+#pragma unroll
+          for (int i = 0; i < KH; ++i) k[i] = *reinterpret_cast<const float4*>(sK + kl * LD + (dl + DL * (half * KH + i)) * 4);
+#pragma unroll
+          for (int r = 0; r < RG; ++r) {
+            float x = 0.f, y = 0.f;
+#pragma unroll
+            for (int i = 0; i < KH; ++i) {
+              const float4 q = *reinterpret_cast<const float4*>(sQ + (rg + r) * HDP + (dl + DL * (half * KH + i)) * 4);
+              x = fmaf(q.x, k[i].x, x);
+              y = fmaf(q.y, k[i].y, y);
+              x = fmaf(q.z, k[i].z, x);
+              y = fmaf(q.w, k[i].w, y);
+            }
+            s[r] += x + y;
+          }
+        }
+        bool far = false;
+#pragma unroll
+        for (int r = 0; r < RG; ++r) {
+          if (DL > 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], 1);
+          if (DL > 2) s[r] += __shfl_xor_sync(0xffffffffu, s[r], 2);
+          bool vis = kl < nk;
+          if (tail) vis &= (rg + r < nr) & sees(a, b, div_group(a, r0 + rg + r), k0 + kl);
+          if (!vis) s[r] = -CUDART_INF_F;
+          if (a.scores && dl == 0 && kl < nk && rg + r < nr)
+            a.scores[(bh * R + r0 + rg + r) * a.sp + (tail ? cur.len : 0) + k0 + kl] = s[r];
+          far |= s[r] > __shfl_sync(0xffffffffu, m, rg + r) + 8.f;
+        }
+        if (__any_sync(0xffffffffu, far)) {                        // the reference of a row moves (as on the tensor cores)
+          moved = true;
+#pragma unroll
+          for (int r = 0; r < RG; ++r) {
+            float x = fmaxf(s[r], __shfl_sync(0xffffffffu, m, rg + r));
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+            if (lane == rg + r && x != -CUDART_INF_F) {
+              al = ex2(m - x);
+              m = x;
+            }
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < RG; ++r) {
+          const float x = __shfl_sync(0xffffffffu, m, rg + r);
+          if (dl == 0) sP[(rg + r) * PL + kl] = ex2(s[r] - (x == -CUDART_INF_F ? 0.f : x));
+        }
+      }
+      __syncwarp();
+      fetch(sK, false);
+      // ---- the row sums, row `lane` --------------------------------------------------------------
+      if (lane < nr) {
+        float x = 0.f, y = 0.f;
+#pragma unroll
+        for (int j = 0; j < NK; j += 4) {
+          const float4 q = *reinterpret_cast<const float4*>(sP + lane * PL + j);
+          x += q.x + q.y;
+          y += q.z + q.w;
+        }
+        l = l * al + (x + y);
+      }
+      if (moved) {
+#pragma unroll
+        for (int r = 0; r < RB; ++r) {
+          const float f = __shfl_sync(0xffffffffu, al, r);
+#pragma unroll
+          for (int c = 0; c < COLS; ++c) o[r][c] *= f;
+        }
+      }
+      cp_async_wait_group<1>();
+      __syncwarp();
+      bool bad = false;
+      if (tail) {
+        if (rb == 0) {
+          constexpr int U = 8;                                     // rows in flight
+          const T* kn = (const T*)a.kn + b * a.kn_b + h * a.kn_h + k0 * a.kn_t;
+          const T* vn = (const T*)a.vn + b * a.vn_b + h * a.vn_h + k0 * a.vn_t;
+          T* kc = (T*)a.kc + b * a.kc_b + h * a.kc_h + (cur.len + k0) * a.kc_s;
+          T* vc = (T*)a.vc + b * a.vc_b + h * a.vc_h + (cur.len + k0) * a.vc_s;
+          const int fit = min(nk, a.S - cur.len - k0);
+          for (int d = lane; d < a.hd; d += 32)
+            for (int r = 0; r < fit; r += U) {
+              T x[U], y[U];
+#pragma unroll
+              for (int i = 0; i < U; ++i)
+                if (r + i < fit) {
+                  x[i] = kn[(r + i) * a.kn_t + d];
+                  y[i] = vn[(r + i) * a.vn_t + d];
+                }
+#pragma unroll
+              for (int i = 0; i < U; ++i)
+                if (r + i < fit) {
+                  kc[(r + i) * a.kc_s + d] = x[i];
+                  vc[(r + i) * a.vc_s + d] = y[i];
+                }
+            }
+          if (a.positions && lane < fit) a.positions[b * a.pos_b + h * a.pos_h + cur.len + k0 + lane] = a.seen[b] + k0 + lane;
+        }
+        // what is not finite must not meet the zero probabilities of rows that do not see it
+        for (int i = lane; i < NK * LD; i += 32) bad |= !isfinite(sV[i]);
+        bad = __any_sync(0xffffffffu, bad);
+        if (bad) {
+          for (int i = lane; i < NK * LD; i += 32)
+            if (!isfinite(sV[i])) sV[i] = 0.f;
+          __syncwarp();
+        }
+      }
+      // ---- output --------------------------------------------------------------------------------
+#pragma unroll 1
+      for (int j = 0; j < NK; j += JS) {
+        float v[JS][COLS];
+#pragma unroll
+        for (int x = 0; x < JS; ++x) {
+          if constexpr (COLS == 2) {
+            *reinterpret_cast<float2*>(v[x]) = *reinterpret_cast<const float2*>(sV + (j + x) * LD + lane * 2);
+          } else {
+#pragma unroll
+            for (int c = 0; c < COLS; c += 4)
+              *reinterpret_cast<float4*>(v[x] + c) = *reinterpret_cast<const float4*>(sV + (j + x) * LD + lane * 4 + c * 32);
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < RB; g += RG) {
+          if (g >= nr) break;
+#pragma unroll
+          for (int r = g; r < g + RG; ++r) {
+            float q[JS];
+            if constexpr (JS == 4) *reinterpret_cast<float4*>(q) = *reinterpret_cast<const float4*>(sP + r * PL + j);
+            else *reinterpret_cast<float2*>(q) = *reinterpret_cast<const float2*>(sP + r * PL + j);
+#pragma unroll
+            for (int x = 0; x < JS; ++x)
+#pragma unroll
+              for (int c = 0; c < COLS; ++c) o[r][c] = fmaf(q[x], v[x][c], o[r][c]);
+          }
+        }
+      }
+      if (bad) {
+        const T* vn = (const T*)a.vn + b * a.vn_b + h * a.vn_h;
+        for (int j = 0; j < nk; ++j) {
+          const unsigned vis = __ballot_sync(0xffffffffu, lane < nr && sees(a, b, div_group(a, r0 + lane), k0 + j));
+#pragma unroll
+          for (int c = 0; c < COLS; ++c) {
+            const int d = COLS == 2 ? lane * 2 + c : lane * 4 + (c & 3) + (c >> 2) * 128;
+            const float x = d < a.hd ? Elem<T>::to(vn[(k0 + j) * a.vn_t + d]) : 0.f;
+            if (isfinite(x)) continue;
+#pragma unroll
+            for (int r = 0; r < RB; ++r)
+              if (vis >> r & 1) o[r][c] += x;
+          }
+        }
+      }
+      __syncwarp();
+      fetch(sV, true);
+    }
+
+    // ---- join the warps: 2 and 3 hand over to 0 and 1, then 1 to 0 --------------------------------
+    auto give = [&](int slot) {
+#pragma unroll
+      for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) sJ[((slot * RB + r) * COLS + c) * 32 + lane] = o[r][c];
+      if (lane < RB) {
+        sM[(slot * RB + lane) * 2] = m;
+        sM[(slot * RB + lane) * 2 + 1] = l;
+      }
+    };
+    auto take = [&](int slot) {
+      float e0 = 1.f, e1 = 0.f;
+      if (lane < RB) {
+        const float m2 = sM[(slot * RB + lane) * 2], x = fmaxf(m, m2);
+        if (x != -CUDART_INF_F) {
+          e0 = ex2(m - x);
+          e1 = ex2(m2 - x);
+        }
+        m = x;
+        l = l * e0 + sM[(slot * RB + lane) * 2 + 1] * e1;
+      }
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        const float f0 = __shfl_sync(0xffffffffu, e0, r), f1 = __shfl_sync(0xffffffffu, e1, r);
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) o[r][c] = o[r][c] * f0 + sJ[((slot * RB + r) * COLS + c) * 32 + lane] * f1;
+      }
+    };
+    if (warp >= 2) give(warp - 2);
+    __syncthreads();
+    if (warp < 2) take(warp);
+    __syncwarp();
+    if (warp == 1) give(1);                                        // only this warp has read slot 1
+    __syncthreads();
+    if (warp == 0) {
+      take(1);
+      const bool first = cur.t == 0, all = first && t1 == cur.n;
+      const long slot = 2L * blockIdx.x + (first ? 1 : 0);
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      if (lane < nr) {
+        if (all && a.lse) a.lse[bh * R + r0 + lane] = lse2(m, l);
+        if (!all) *reinterpret_cast<float2*>(a.part_ml + (slot * a.rows + lane) * 2) = make_float2(m, l);
+      }
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        const float f = __shfl_sync(0xffffffffu, inv, r);
+        if (r >= nr) continue;
+        const int tok = div_group(a, r0 + r);
+        T* po = (T*)a.o + (((long)b * a.T + tok) * a.nkv * a.group + h * a.group + r0 + r - tok * a.group) * a.hd;
+        float* pp = a.part_o + (slot * a.rows + r) * a.hd;
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) {
+          const int d = COLS == 2 ? lane * 2 + c : lane * 4 + (c & 3) + (c >> 2) * 128;
+          if (d >= a.hd) continue;
+          if (all) po[d] = Elem<T>::of(o[r][c] * f);
+          else pp[d] = o[r][c];
         }
       }
     }
-    __syncthreads();
-    for (int r = 0; r < nr; ++r) {
-      const int row = r0 + r, t = row / a.group, g = row - t * a.group;
-#pragma unroll
-      for (int c = 0; c < GC; ++c) {
-        const int d = tid + c * GT;
-        if (d >= hd) continue;
-        if (first && last)
-          ((T*)a.o)[(((long)b * a.T + t) * a.nkv * a.group + h * a.group + g) * hd + d] = Elem<T>::of(acc[c][r] * sA[r]);
-        else
-          a.part_o[(slot * a.rows + r) * hd + d] = acc[c][r];
-      }
-    }
-    __syncthreads();
-    w += t1 - sg.t0;
+    done = end;
+    cur.t = 0;
+    cur_next_unit(cur, a, NK);
   }
 }
 
@@ -214,17 +401,17 @@ __global__ void __launch_bounds__(JT) kv_join_k(KvAttnArgs a, int row_blocks) {
   const int b = (int)(bh / a.nkv), h = (int)(bh - (long)b * a.nkv);
   join_wait();
   Plan plan{0, 1};
-  int n = 1;
-  long ub = 0;                                      // first tile of row block 0
+  int n = 1 + a.extra;                              // costs of a row block
+  long ub = 0;                                      // cost of the first tile of row block 0
   if (!a.whole) {
     plan = make_plan(a, a.prefix[a.B], a.ctas, a.min_per);
     const int p0 = a.prefix[b];
     n = a.prefix[b + 1] - p0;
-    ub = (long)p0 * a.nkv * a.nrb + (long)h * a.nrb * n;
+    ub = (long)p0 * a.nkv * a.nrb + (long)h * a.nrb * n + a.extra;
   }
   auto pieces = [&](int rb) {
     const long s = ub + (long)rb * n;
-    return Pieces{s / plan.per, (s + n - 1) / plan.per};
+    return Pieces{s / plan.per, (s + n - a.extra - 1) / plan.per};
   };
   if (out) {
     const int row = (int)(min(idx, total - 1) - bh * R), rb = row / a.rows, r = row - rb * a.rows;
@@ -298,13 +485,26 @@ __global__ void __launch_bounds__(JT) kv_join_k(KvAttnArgs a, int row_blocks) {
     if (j0 + i * JT + tid < hi) wt[i * JT + tid] += add[i];
 }
 
+template <typename T, int HDP, int RB>
+int run_any(const KvAttnArgs& a, cudaStream_t st) {
+  const size_t sm = std::max(simt_bytes<HDP, RB>(), (size_t)(a.B + 33) * 4);
+  const cudaError_t e = cudaFuncSetAttribute(kv_attn_any_k<T, HDP, RB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
+  if (e != cudaSuccess) return (int)e;
+  kv_attn_any_k<T, HDP, RB><<<a.whole ? a.B * a.nkv * a.nrb : a.ctas, 32 * SW, sm, st>>>(a, a.ctas);
+  return (int)cudaGetLastError();
+}
+template <typename T, int HDP>
+int run_any_rows(const KvAttnArgs& a, cudaStream_t st) {
+  if (a.rows == 1) return run_any<T, HDP, 1>(a, st);
+  if constexpr (sizeof(T) == 4 && most_rows<HDP>() > 8) {
+    if (a.rows > 8) return run_any<T, HDP, most_rows<HDP>()>(a, st);
+  }
+  return run_any<T, HDP, 8>(a, st);
+}
 template <typename T>
 int launch(const KvAttnArgs& a, cudaStream_t st) {
-  const size_t sm = (size_t)(GR * a.hd + GK * (a.hd | 1) + GR * GK + 2 * GR) * 4 + (size_t)(a.B + 33) * 4;
-  const cudaError_t e = cudaFuncSetAttribute(kv_attn_any_k<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
-  if (e != cudaSuccess) return (int)e;
-  kv_attn_any_k<T><<<a.ctas, GT, sm, st>>>(a);
-  return (int)cudaGetLastError();
+  return a.hd <= 64 ? run_any_rows<T, 64>(a, st) : a.hd <= 128 ? run_any_rows<T, 128>(a, st)
+         : a.hd <= 256 ? run_any_rows<T, 256>(a, st) : run_any_rows<T, 512>(a, st);
 }
 
 template <typename T>
@@ -325,14 +525,20 @@ int join(const KvAttnArgs& a, cudaStream_t st) {
 void kv_attn_plan(KvAttnArgs& a, int dtype, int sms) {
   a.tc = kv_attn_tc_takes(a, dtype);
   if (a.tc) return kv_attn_tc_plan(a, sms);
-  const size_t sm = (size_t)(s0::kv::GR * a.hd + s0::kv::GK * (a.hd | 1) + s0::kv::GR * s0::kv::GK) * 4;
+  using namespace s0::kv;
   const int R = a.T * a.group;
-  a.rows = s0::kv::GR;
+  const int most = dtype ? 8 : a.hd <= 64 ? most_rows<64>() : a.hd <= 128 ? most_rows<128>() : most_rows<256>();
+  a.rows = R == 1 ? 1 : R <= 8 ? 8 : most;
   a.nrb = (R + a.rows - 1) / a.rows;
-  a.tile = s0::kv::GK;
-  a.min_per = 4;
+  a.tile = a.hd <= 64 ? slab_keys<64>() : a.hd <= 128 ? slab_keys<128>() : slab_keys<256>();
+  a.min_per = SW;
   a.whole = 0;
-  a.ctas = sms * (int)std::max<size_t>(1, std::min<size_t>(8, (size_t)200 * 1024 / sm));
+  a.extra = 2;
+  a.ctas = (a.hd > 256 ? 1 : 2) * sms;
+  bool vec = dtype == 0 && a.hd % 4 == 0;
+  for (long s : {a.kn_b, a.kn_t, a.kn_h, a.vn_b, a.vn_t, a.vn_h, a.kc_b, a.kc_h, a.kc_s, a.vc_b, a.vc_h, a.vc_s}) vec = vec && s % 4 == 0;
+  for (const void* p : {a.kn, a.vn, (const void*)a.kc, (const void*)a.vc}) vec = vec && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+  a.vec = vec;
 }
 
 int kv_attn_launch(const KvAttnArgs& a, int dtype, cudaStream_t st) {

@@ -7,6 +7,10 @@
 // whole is written out by it; one that several share leaves partial results (unnormalised output,
 // running maximum and sum), which a second kernel joins.  A CTA has at most two such pieces: the
 // end of one unit (slot 2 c) and the beginning of another (slot 2 c + 1).
+//
+// A unit costs something of its own (queries, the mask, the new rows, its output), which counts as
+// `a.extra` tiles at its beginning: the line is one of costs.  A CTA whose share begins within them
+// begins with tile 0, so tile t of a unit whose costs begin at s is CTA (s + extra + t) / per's.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -38,14 +42,14 @@ S0_DEV int cached(const KvAttnArgs& a, int b) { return min(max(__ldg(a.lengths +
 // key tiles of a sequence: its cached tokens, then the new ones (tiles never mix the two)
 S0_DEV int tiles_of(const KvAttnArgs& a, int len, int KT) { return (len + KT - 1) / KT + (a.T + KT - 1) / KT; }
 
-// s_pre[b] = tiles of one (head, row block) before sequence b; returns the total.  Called by all
+// s_pre[b] = costs of one (head, row block) before sequence b; returns the total.  Called by all
 // threads of the block; needs B + 1 + 32 ints of shared memory.
 S0_DEV long plan_prefix(const KvAttnArgs& a, int KT, int* s_pre) {
   int* s_w = s_pre + a.B + 1;
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5;
   const int per = (a.B + nt - 1) / nt, b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
   int sum = 0;
-  for (int b = b0; b < b1; ++b) sum += tiles_of(a, cached(a, b), KT);
+  for (int b = b0; b < b1; ++b) sum += tiles_of(a, cached(a, b), KT) + a.extra;
   int inc = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -59,7 +63,7 @@ S0_DEV long plan_prefix(const KvAttnArgs& a, int KT, int* s_pre) {
   int run = base + inc - sum;
   for (int b = b0; b < b1; ++b) {
     s_pre[b] = run;
-    run += tiles_of(a, cached(a, b), KT);
+    run += tiles_of(a, cached(a, b), KT) + a.extra;
   }
   if (b1 == a.B && b0 < a.B) s_pre[a.B] = run;
   __syncthreads();
@@ -67,39 +71,14 @@ S0_DEV long plan_prefix(const KvAttnArgs& a, int KT, int* s_pre) {
 }
 
 struct Plan {
-  long total;  // tiles of all units
-  long per;    // tiles of a CTA
+  long total;  // costs of all units
+  long per;    // costs of a CTA
 };
-S0_DEV Plan make_plan(const KvAttnArgs& a, long tiles, int ctas, int min_per) {
+S0_DEV Plan make_plan(const KvAttnArgs& a, long costs, int ctas, int min_per) {
   Plan p;
-  p.total = tiles * a.nkv * a.nrb;
+  p.total = costs * a.nkv * a.nrb;
   p.per = max((long)min_per, (p.total + ctas - 1) / ctas);
   return p;
-}
-
-// the unit that tile w of the whole line belongs to
-struct Seg {
-  int b, h, rb;  // sequence, key head, row block
-  int len, n;    // cached tokens, tiles of the unit
-  int t0;        // tile w within the unit
-};
-S0_DEV Seg find_seg(const KvAttnArgs& a, const int* s_pre, long w, int KT) {
-  const long hr = (long)a.nkv * a.nrb;
-  int lo = 0, hi = a.B - 1;
-  while (lo < hi) {  // the last b with pre[b] * hr <= w
-    const int mid = (lo + hi + 1) >> 1;
-    if ((long)s_pre[mid] * hr <= w) lo = mid; else hi = mid - 1;
-  }
-  Seg s;
-  s.b = lo;
-  s.len = cached(a, lo);
-  s.n = s_pre[lo + 1] - s_pre[lo];
-  const long rem = w - (long)s_pre[lo] * hr;
-  const int u = (int)(rem / s.n);
-  s.t0 = (int)(rem - (long)u * s.n);
-  s.h = u / a.nrb;
-  s.rb = u - s.h * a.nrb;
-  return s;
 }
 
 // row / group for rows below 2^20: (row + 1/2) / group is at least 1 / (2 group) away from an integer
@@ -145,6 +124,25 @@ S0_DEV bool cur_skip(Cur& c, const KvAttnArgs& a, int KT, int by) {
   return false;
 }
 
+// The unit and tile at cost w of the line; returns how many tiles lie before it.
+S0_DEV long find_tile(Cur& c, const KvAttnArgs& a, const int* s_pre, long w) {
+  const long hr = (long)a.nkv * a.nrb;
+  int lo = 0, hi = a.B - 1;
+  while (lo < hi) {  // the last b with pre[b] * hr <= w
+    const int mid = (lo + hi + 1) >> 1;
+    if ((long)s_pre[mid] * hr <= w) lo = mid; else hi = mid - 1;
+  }
+  const long rem = w - (long)s_pre[lo] * hr;
+  const int cost = s_pre[lo + 1] - s_pre[lo];
+  c.b = lo;
+  c.len = cached(a, lo);
+  c.n = cost - a.extra;
+  c.u = (int)(rem / cost);
+  const int x = (int)(rem - (long)c.u * cost);
+  c.t = max(0, x - a.extra);
+  return w - ((long)lo * hr + c.u) * a.extra - min(x, a.extra);
+}
+
 // The first tile of this CTA and how many it has.  a.whole: one unit per CTA (caches that are short
 // enough); otherwise the even split, whose prefix table CTA 0 leaves for the join.
 S0_DEV long cta_share(Cur& c, const KvAttnArgs& a, int KT, int* scratch, int ctas) {
@@ -159,15 +157,10 @@ S0_DEV long cta_share(Cur& c, const KvAttnArgs& a, int KT, int* scratch, int cta
   const Plan p = make_plan(a, plan_prefix(a, KT, scratch), ctas, a.min_per);
   if (blockIdx.x == 0)
     for (int i = threadIdx.x; i <= a.B; i += blockDim.x) a.prefix[i] = scratch[i];
-  const long w = (long)blockIdx.x * p.per;
-  if (w >= p.total) return 0;
-  const Seg s = find_seg(a, scratch, w, KT);
-  c.b = s.b;
-  c.u = s.h * a.nrb + s.rb;
-  c.len = s.len;
-  c.n = s.n;
-  c.t = s.t0;
-  return min(p.total - w, p.per);
+  const long w0 = (long)blockIdx.x * p.per, w1 = w0 + p.per;
+  if (w0 >= p.total) return 0;
+  const long end = w1 < p.total ? find_tile(c, a, scratch, w1) : p.total - (long)a.B * hr * a.extra;
+  return end - find_tile(c, a, scratch, w0);
 }
 
 // Programmatic launch: the kernel behind this one may be set up while it runs, and waits for its results.

@@ -413,7 +413,8 @@ __global__ void __launch_bounds__(32 * WARPS, per_sm<WR>()) kv_attn_tc_k(KvAttnA
         __syncwarp();
         if (warp == 1) give(1);                                 // only this warp has read slot 1
         __syncthreads();
-        if (warp == 0) take(1);                                 // slot 0 is free from here, slot 1 after the next barrier
+        if (warp == 0) take(1);
+        __syncthreads();                                        // the next unit may end at once for warp 3
       } else {
         if (group == 1) give(wr);
         __syncthreads();
@@ -496,6 +497,7 @@ void kv_attn_tc_plan(KvAttnArgs& a, int sms) {
   a.ctas = (wr == WARPS ? per_sm<WARPS>() : per_sm<1>()) * sms;
   a.min_per = WARPS / wr;
   a.whole = 0;
+  a.extra = 2;
 }
 
 int kv_attn_tc_launch(const KvAttnArgs& a, int dtype, cudaStream_t st) {

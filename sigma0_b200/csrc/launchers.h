@@ -371,9 +371,9 @@ struct KvAttnArgs {
   long mask_b, wt_b, wt_h, pos_b, pos_h;  // mask_b 0: one mask for all sequences
   int B, T, nkv, group, hd, S;
   float scale_log2;                   // softmax scale * log2(e)
-  // set by kv_attn_plan: rows of a block, row blocks, keys of a tile, CTAs, least tiles of a CTA, one
-  // CTA per unit (no split), tensor cores
-  int rows, nrb, tile, ctas, min_per, whole, tc;
+  // set by kv_attn_plan: rows of a block, row blocks, keys of a tile, CTAs, least cost of a CTA, cost of a
+  // unit besides its tiles, one CTA per unit (no split), tensor cores, 16-byte loads of floats
+  int rows, nrb, tile, ctas, min_per, extra, whole, tc, vec;
   // scratch: 2 * ctas pieces of [rows, hd] and [rows, 2]; with weights [B, nkv, T * group, sp] scores
   // and [B, nkv, T * group] log-sum-exps
   float *part_o, *part_ml, *scores, *lse;
