@@ -113,10 +113,43 @@ __global__ void __launch_bounds__(32 * SW, HDP == 512 ? 1 : 2) kv_attn_any_k(KvA
     const int ncache = (cur.len + NK - 1) / NK;
     const long end = done + (t1 - cur.t);
     __syncthreads();                                               // the last unit's queries have been read
-    for (int i = tid; i < RB * HDP; i += 32 * SW) {
-      const int r = i / HDP, d = i % HDP, tok = div_group(a, r0 + r);
-      sQ[i] = r < nr && d < a.hd ? Elem<T>::to(((const T*)a.q)[b * a.q_b + tok * a.q_t + (long)(h * a.group + r0 + r - tok * a.group) * a.q_h + d]) * a.scale_log2
-                                 : 0.f;
+    constexpr int QN = RB * HDP / (32 * SW) > 0 ? RB * HDP / (32 * SW) : 1, QB = QN < 8 ? QN : 8;   // loads in flight
+    for (int i0 = tid; i0 < RB * HDP; i0 += 32 * SW * QB) {
+      float x[QB];
+#pragma unroll
+      for (int k = 0; k < QB; ++k) {
+        const int i = i0 + 32 * SW * k, r = i / HDP, d = i % HDP, tok = div_group(a, r0 + r);
+        x[k] = r < nr && d < a.hd ? Elem<T>::to(((const T*)a.q)[b * a.q_b + tok * a.q_t + (long)(h * a.group + r0 + r - tok * a.group) * a.q_h + d]) : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < QB; ++k)
+        if (i0 + 32 * SW * k < RB * HDP) sQ[i0 + 32 * SW * k] = x[k] * a.scale_log2;
+    }
+    if (t1 == cur.n && rb == 0) {                                  // the new rows go behind the cached ones
+      constexpr int U = 8;                                         // rows in flight per warp
+      const T* kn = (const T*)a.kn + b * a.kn_b + h * a.kn_h;
+      const T* vn = (const T*)a.vn + b * a.vn_b + h * a.vn_h;
+      T* kc = (T*)a.kc + b * a.kc_b + h * a.kc_h + cur.len * a.kc_s;
+      T* vc = (T*)a.vc + b * a.vc_b + h * a.vc_h + cur.len * a.vc_s;
+      const int fit = min(a.T, a.S - cur.len);
+      for (int d = lane; d < a.hd; d += 32)
+        for (int r = warp; r < fit; r += U * SW) {
+          T x[U], y[U];
+#pragma unroll
+          for (int i = 0; i < U; ++i)
+            if (r + i * SW < fit) {
+              x[i] = kn[(r + i * SW) * a.kn_t + d];
+              y[i] = vn[(r + i * SW) * a.vn_t + d];
+            }
+#pragma unroll
+          for (int i = 0; i < U; ++i)
+            if (r + i * SW < fit) {
+              kc[(r + i * SW) * a.kc_s + d] = x[i];
+              vc[(r + i * SW) * a.vc_s + d] = y[i];
+            }
+        }
+      if (a.positions)
+        for (int r = tid; r < fit; r += 32 * SW) a.positions[b * a.pos_b + h * a.pos_h + cur.len + r] = a.seen[b] + r;
     }
     __syncthreads();
     float o[RB][COLS];
@@ -215,33 +248,11 @@ __global__ void __launch_bounds__(32 * SW, HDP == 512 ? 1 : 2) kv_attn_any_k(KvA
       __syncwarp();
       bool bad = false;
       if (tail) {
-        if (rb == 0) {
-          constexpr int U = 8;                                     // rows in flight
-          const T* kn = (const T*)a.kn + b * a.kn_b + h * a.kn_h + k0 * a.kn_t;
-          const T* vn = (const T*)a.vn + b * a.vn_b + h * a.vn_h + k0 * a.vn_t;
-          T* kc = (T*)a.kc + b * a.kc_b + h * a.kc_h + (cur.len + k0) * a.kc_s;
-          T* vc = (T*)a.vc + b * a.vc_b + h * a.vc_h + (cur.len + k0) * a.vc_s;
-          const int fit = min(nk, a.S - cur.len - k0);
-          for (int d = lane; d < a.hd; d += 32)
-            for (int r = 0; r < fit; r += U) {
-              T x[U], y[U];
-#pragma unroll
-              for (int i = 0; i < U; ++i)
-                if (r + i < fit) {
-                  x[i] = kn[(r + i) * a.kn_t + d];
-                  y[i] = vn[(r + i) * a.vn_t + d];
-                }
-#pragma unroll
-              for (int i = 0; i < U; ++i)
-                if (r + i < fit) {
-                  kc[(r + i) * a.kc_s + d] = x[i];
-                  vc[(r + i) * a.vc_s + d] = y[i];
-                }
-            }
-          if (a.positions && lane < fit) a.positions[b * a.pos_b + h * a.pos_h + cur.len + k0 + lane] = a.seen[b] + k0 + lane;
-        }
         // what is not finite must not meet the zero probabilities of rows that do not see it
-        for (int i = lane; i < NK * LD; i += 32) bad |= !isfinite(sV[i]);
+        for (int i = lane * 4; i < NK * LD; i += 128) {
+          const float4 x = *reinterpret_cast<const float4*>(sV + i);
+          bad |= !(isfinite(x.x) && isfinite(x.y) && isfinite(x.z) && isfinite(x.w));
+        }
         bad = __any_sync(0xffffffffu, bad);
         if (bad) {
           for (int i = lane; i < NK * LD; i += 32)
@@ -533,7 +544,7 @@ void kv_attn_plan(KvAttnArgs& a, int dtype, int sms) {
   a.tile = a.hd <= 64 ? slab_keys<64>() : a.hd <= 128 ? slab_keys<128>() : slab_keys<256>();
   a.min_per = SW;
   a.whole = 0;
-  a.extra = 2;
+  a.extra = SW;
   a.ctas = (a.hd > 256 ? 1 : 2) * sms;
   bool vec = dtype == 0 && a.hd % 4 == 0;
   for (long s : {a.kn_b, a.kn_t, a.kn_h, a.vn_b, a.vn_t, a.vn_h, a.kc_b, a.kc_h, a.kc_s, a.vc_b, a.vc_h, a.vc_s}) vec = vec && s % 4 == 0;

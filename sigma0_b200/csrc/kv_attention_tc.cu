@@ -497,7 +497,7 @@ void kv_attn_tc_plan(KvAttnArgs& a, int sms) {
   a.ctas = (wr == WARPS ? per_sm<WARPS>() : per_sm<1>()) * sms;
   a.min_per = WARPS / wr;
   a.whole = 0;
-  a.extra = 2;
+  a.extra = 3;
 }
 
 int kv_attn_tc_launch(const KvAttnArgs& a, int dtype, cudaStream_t st) {
