@@ -782,12 +782,15 @@ static void kv_slots(const at::Tensor& t, const char* name, at::ScalarType dt, c
   TORCH_CHECK(t.sizes() == kc.sizes().slice(0, kc.dim() - 1) && (t.stride(-1) == 1 || t.size(-1) <= 1), name,
               " must have the cache's shape without the head dimension, slots contiguous");
 }
-static void kv_caches(const at::Tensor& kc, const at::Tensor& vc, int64_t dim) {
+// a cache [B, nkv, S, hd] is one of a single layer
+static int64_t kv_layers(const at::Tensor& t, int64_t rank) { return t.dim() == rank ? t.size(0) : 1; }
+static int64_t kv_layer_stride(const at::Tensor& t, int64_t rank) { return t.dim() == rank ? t.stride(0) : 0; }
+static void kv_caches(const at::Tensor& kc, const at::Tensor& vc, bool layers) {
   TORCH_CHECK(kc.is_cuda() && vc.device() == kc.device(), "the caches must be CUDA tensors of one device");
   kv_dtype(kc, "k_cache");
   TORCH_CHECK(kc.scalar_type() == vc.scalar_type(), "the caches must have one dtype");
-  TORCH_CHECK(kc.dim() == dim && kc.sizes() == vc.sizes(), "the caches must have one shape [",
-              dim == 5 ? "layers, " : "", "B, kv heads, slots, head dim]");
+  TORCH_CHECK((kc.dim() == 4 || (layers && kc.dim() == 5)) && kc.sizes() == vc.sizes(), "the caches must have one shape [",
+              layers ? "(layers,) " : "", "B, kv heads, slots, head dim]");
   TORCH_CHECK(kc.stride(-1) == 1 && vc.stride(-1) == 1, "the caches' head dimension must be contiguous");
   TORCH_CHECK(kc.size(-1) >= 1 && kc.size(-2) * kc.size(-1) < (int64_t)1 << 31, "a head's slots x channels must stay below 2^31");
 }
@@ -795,7 +798,7 @@ static void kv_caches(const at::Tensor& kc, const at::Tensor& vc, int64_t dim) {
 at::Tensor kv_attn(at::Tensor q, at::Tensor kn, at::Tensor vn, at::Tensor kc, at::Tensor vc, at::Tensor lengths,
                    c10::optional<at::Tensor> mask, double scale, c10::optional<at::Tensor> weight,
                    c10::optional<at::Tensor> positions, c10::optional<at::Tensor> seen) {
-  kv_caches(kc, vc, 4);
+  kv_caches(kc, vc, false);
   const auto dev = kc.device();
   const int dt = kv_dtype(kc, "k_cache");
   const int64_t B = kc.size(0), nkv = kc.size(1), S = kc.size(2), hd = kc.size(3);
@@ -851,7 +854,7 @@ at::Tensor kv_attn(at::Tensor q, at::Tensor kn, at::Tensor vn, at::Tensor kc, at
   a.scale_log2 = (float)(scale * 1.4426950408889634);
   a.inv_group = 1.f / (float)a.group;
   kv_attn_plan(a, dt, num_sms(kc));
-  TORCH_CHECK(B * nh * T < (int64_t)1 << 30 && B * nkv * ((S + T) / 2048 + 1) < (int64_t)1 << 30, "too many heads and rows");
+  TORCH_CHECK(B * nh * T < (int64_t)1 << 30 && B * nkv * ((S + T) / 1024 + 1) < (int64_t)1 << 30, "too many heads and rows");
   const auto f32 = q.options().dtype(at::kFloat);
   // one scratch tensor: pieces [2 ctas, rows, hd + 2], then with weights the scores and row sums
   const int64_t po = 2LL * a.ctas * a.rows * hd, ml = 4LL * a.ctas * a.rows, R = T * (nh / nkv);
@@ -874,9 +877,9 @@ std::vector<at::Tensor> kv_evict(at::Tensor kc, at::Tensor vc, at::Tensor weight
                                  at::Tensor lengths, at::Tensor seen, int64_t keep, int64_t recent, int64_t sinks,
                                  c10::optional<at::Tensor> weight_out, c10::optional<at::Tensor> positions_out,
                                  c10::optional<at::Tensor> lengths_out) {
-  kv_caches(kc, vc, 5);
+  kv_caches(kc, vc, true);
   const auto dev = kc.device();
-  const int64_t N = kc.size(0), B = kc.size(1), nkv = kc.size(2), S = kc.size(3), hd = kc.size(4);
+  const int64_t N = kv_layers(kc, 5), B = kc.size(-4), nkv = kc.size(-3), S = kc.size(-2), hd = kc.size(-1);
   kv_slots(weight, "weight", at::kFloat, kc);
   kv_slots(positions, "positions", at::kInt, kc);
   kv_ints(lengths, "lengths", B, dev);
@@ -902,12 +905,12 @@ std::vector<at::Tensor> kv_evict(at::Tensor kc, at::Tensor vc, at::Tensor weight
   a.weight = weight.data_ptr<float>(); a.positions = positions.data_ptr<int>();
   a.lengths = lengths.data_ptr<int>(); a.seen = seen.data_ptr<int>();
   a.weight_out = wo.data_ptr<float>(); a.positions_out = po.data_ptr<int>(); a.lengths_out = lo.data_ptr<int>();
-  a.kc_n = kc.stride(0); a.kc_b = kc.stride(1); a.kc_h = kc.stride(2); a.kc_s = kc.stride(3);
-  a.vc_n = vc.stride(0); a.vc_b = vc.stride(1); a.vc_h = vc.stride(2); a.vc_s = vc.stride(3);
-  a.w_n = weight.stride(0); a.w_b = weight.stride(1); a.w_h = weight.stride(2);
-  a.p_n = positions.stride(0); a.p_b = positions.stride(1); a.p_h = positions.stride(2);
-  a.wo_n = wo.stride(0); a.wo_b = wo.stride(1); a.wo_h = wo.stride(2);
-  a.po_n = po.stride(0); a.po_b = po.stride(1); a.po_h = po.stride(2);
+  a.kc_n = kv_layer_stride(kc, 5); a.kc_b = kc.stride(-4); a.kc_h = kc.stride(-3); a.kc_s = kc.stride(-2);
+  a.vc_n = kv_layer_stride(vc, 5); a.vc_b = vc.stride(-4); a.vc_h = vc.stride(-3); a.vc_s = vc.stride(-2);
+  a.w_n = kv_layer_stride(weight, 4); a.w_b = weight.stride(-3); a.w_h = weight.stride(-2);
+  a.p_n = kv_layer_stride(positions, 4); a.p_b = positions.stride(-3); a.p_h = positions.stride(-2);
+  a.wo_n = kv_layer_stride(wo, 4); a.wo_b = wo.stride(-3); a.wo_h = wo.stride(-2);
+  a.po_n = kv_layer_stride(po, 4); a.po_b = po.stride(-3); a.po_h = po.stride(-2);
   a.N = (int)N; a.B = (int)B; a.nkv = (int)nkv; a.S = (int)S; a.hd = (int)hd; a.esize = (int)kc.element_size();
   a.keep = (int)cap; a.recent = (int)std::min(recent, cap); a.sinks = (int)std::min(sinks, cap);
   a.moves = reinterpret_cast<int2*>(ws.data_ptr<int>());
@@ -921,9 +924,9 @@ std::vector<at::Tensor> kv_evict(at::Tensor kc, at::Tensor vc, at::Tensor weight
 std::vector<at::Tensor> kv_commit(at::Tensor parents, at::Tensor tokens, at::Tensor targets, at::Tensor kc, at::Tensor vc,
                                   at::Tensor lengths, c10::optional<at::Tensor> weight,
                                   c10::optional<at::Tensor> positions, c10::optional<at::Tensor> seen) {
-  kv_caches(kc, vc, 5);
+  kv_caches(kc, vc, true);
   const auto dev = kc.device();
-  const int64_t N = kc.size(0), B = kc.size(1), nkv = kc.size(2), S = kc.size(3), hd = kc.size(4);
+  const int64_t N = kv_layers(kc, 5), B = kc.size(-4), nkv = kc.size(-3), S = kc.size(-2), hd = kc.size(-1);
   req(tokens, at::kLong, "tokens");
   req(targets, at::kLong, "targets");
   TORCH_CHECK(tokens.dim() == 2 && tokens.size(0) == B && targets.sizes() == tokens.sizes() && tokens.device() == dev &&
@@ -938,14 +941,14 @@ std::vector<at::Tensor> kv_commit(at::Tensor parents, at::Tensor tokens, at::Ten
   if (weight && weight->defined()) {
     kv_slots(*weight, "weight", at::kFloat, kc);
     a.weight = weight->data_ptr<float>();
-    a.w_n = weight->stride(0); a.w_b = weight->stride(1); a.w_h = weight->stride(2);
+    a.w_n = kv_layer_stride(*weight, 4); a.w_b = weight->stride(-3); a.w_h = weight->stride(-2);
   }
   if (positions && positions->defined()) {
     kv_slots(*positions, "positions", at::kInt, kc);
     TORCH_CHECK(seen && seen->defined(), "positions need seen");
     kv_ints(*seen, "seen", B, dev);
     a.positions = positions->data_ptr<int>();
-    a.p_n = positions->stride(0); a.p_b = positions->stride(1); a.p_h = positions->stride(2);
+    a.p_n = kv_layer_stride(*positions, 4); a.p_b = positions->stride(-3); a.p_h = positions->stride(-2);
     a.seen = seen->data_ptr<int>();
   }
   c10::cuda::CUDAGuard guard(dev);
@@ -961,8 +964,8 @@ std::vector<at::Tensor> kv_commit(at::Tensor parents, at::Tensor tokens, at::Ten
   a.path = path.data_ptr<int>(); a.count = count.data_ptr<int>();
   a.next = reinterpret_cast<long*>(next.data_ptr<int64_t>());
   a.par_b = parents.dim() == 2 ? T : 0;
-  a.kc_n = kc.stride(0); a.kc_b = kc.stride(1); a.kc_h = kc.stride(2); a.kc_s = kc.stride(3);
-  a.vc_n = vc.stride(0); a.vc_b = vc.stride(1); a.vc_h = vc.stride(2); a.vc_s = vc.stride(3);
+  a.kc_n = kv_layer_stride(kc, 5); a.kc_b = kc.stride(-4); a.kc_h = kc.stride(-3); a.kc_s = kc.stride(-2);
+  a.vc_n = kv_layer_stride(vc, 5); a.vc_b = vc.stride(-4); a.vc_h = vc.stride(-3); a.vc_s = vc.stride(-2);
   a.N = (int)N; a.B = (int)B; a.T = (int)T; a.nkv = (int)nkv; a.S = (int)S; a.hd = (int)hd;
   a.esize = (int)kc.element_size();
   const int rc = kv_commit_launch(a, stream());

@@ -375,8 +375,10 @@ __global__ void __launch_bounds__(32 * SW, HDP == 512 ? 1 : 2) kv_attn_any_k(KvA
 }
 
 // Joins the pieces of the units that several CTAs share, and adds up the weights.  Blocks
-// [0, B heads T): one row's output; the others: JW slots of one (sequence, key head) each.
-constexpr int JT = 256, JW = 2048;
+// [0, row_blocks): rows of the output; the others: JT PER slots of one (sequence, key head) each.
+constexpr int JT = 256;
+// slots of a thread and rows at a time: one row wants many slots in flight, many rows share fewer
+constexpr int slots_of(int rows) { return rows < 4 ? 8 : 4; }
 
 struct Pieces {
   long c0, c1;  // first and last CTA of the unit
@@ -400,8 +402,9 @@ S0_DEV void row_sum(const KvAttnArgs& a, const Pieces& p, int r, float& M, float
 }
 
 // WPR warps share the pieces of a row
-template <typename T, int WPR>
+template <typename T, int WPR, int PER>
 __global__ void __launch_bounds__(JT) kv_join_k(KvAttnArgs a, int row_blocks) {
+  constexpr int JW = JT * PER, UR = PER == 4 ? 4 : 1;
   constexpr int RPB = JT / 32 / WPR, COLS = 4;     // rows of a block, columns of a lane at a time
   __shared__ float s_x[JT * COLS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, R = a.T * a.group;
@@ -463,9 +466,22 @@ __global__ void __launch_bounds__(JT) kv_join_k(KvAttnArgs a, int row_blocks) {
     }
     return;
   }
+  // weights: what does not depend on the row sums is loaded before they are known
   const int hi = min(a.S, cached(a, b) + a.T), j0 = (wb - (int)bh * nch) * JW;
   if (j0 >= hi) return;
-  float add[JW / JT] = {};
+  float* wt = a.weight + b * a.wt_b + h * a.wt_h + j0;
+  const float* sc = a.scores + bh * R * a.sp + j0;
+  float add[PER] = {}, was[PER], s[UR][PER];
+  auto load = [&](int q0) {
+#pragma unroll
+    for (int q = 0; q < UR; ++q)
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        s[q][i] = q0 + q < R && j0 + i * JT + tid < hi ? sc[(q0 + q) * a.sp + i * JT + tid] : -CUDART_INF_F;
+  };
+#pragma unroll
+  for (int i = 0; i < PER; ++i) was[i] = j0 + i * JT + tid < hi ? wt[i * JT + tid] : 0.f;
+  load(0);
   for (int q0 = 0; q0 < R; q0 += JT) {
     __syncthreads();
     for (int q = warp; q < min(JT, R - q0); q += JT / 32) {
@@ -482,18 +498,20 @@ __global__ void __launch_bounds__(JT) kv_join_k(KvAttnArgs a, int row_blocks) {
       if (lane == 0) s_x[q] = x;
     }
     __syncthreads();
-    for (int q = 0; q < min(JT, R - q0); ++q) {
-      const float* sc = a.scores + (bh * R + q0 + q) * a.sp + j0;
-      const float ls = s_x[q];
+    for (int q = 0; q < min(JT, R - q0); q += UR) {
+      float e[UR];
 #pragma unroll
-      for (int i = 0; i < JW / JT; ++i)
-        if (j0 + i * JT + tid < hi) add[i] += ex2(sc[i * JT + tid] - ls);
+      for (int k = 0; k < UR; ++k) e[k] = q + k < JT && q0 + q + k < R ? s_x[q + k] : CUDART_INF_F;
+      if (q0 + q > 0) load(q0 + q);
+#pragma unroll
+      for (int k = 0; k < UR; ++k)
+#pragma unroll
+        for (int i = 0; i < PER; ++i) add[i] += q0 + q + k < R ? ex2(s[k][i] - e[k]) : 0.f;
     }
   }
-  float* wt = a.weight + b * a.wt_b + h * a.wt_h + j0;
 #pragma unroll
-  for (int i = 0; i < JW / JT; ++i)
-    if (j0 + i * JT + tid < hi) wt[i * JT + tid] += add[i];
+  for (int i = 0; i < PER; ++i)
+    if (j0 + i * JT + tid < hi) wt[i * JT + tid] = was[i] + add[i];
 }
 
 template <typename T, int HDP, int RB>
@@ -518,16 +536,20 @@ int launch(const KvAttnArgs& a, cudaStream_t st) {
          : a.hd <= 256 ? run_any_rows<T, 256>(a, st) : run_any_rows<T, 512>(a, st);
 }
 
-template <typename T>
-int join(const KvAttnArgs& a, cudaStream_t st) {
+template <typename T, int PER>
+int join_rows(const KvAttnArgs& a, cudaStream_t st) {
   // few rows leave room for a block each, whose warps take turns at the pieces
   const long rows = a.whole ? 0 : (long)a.B * a.nkv * a.T * a.group;
-  const bool wide = rows > 4L * a.ctas;
+  const bool wide = rows > a.ctas;
   const long row_blocks = wide ? (rows + JT / 32 - 1) / (JT / 32) : rows;
-  const long blocks = row_blocks + (a.weight ? (long)a.B * a.nkv * ((a.S + a.T + JW - 1) / JW) : 0);
+  const long blocks = row_blocks + (a.weight ? (long)a.B * a.nkv * ((a.S + a.T + JT * PER - 1) / (JT * PER)) : 0);
   if (blocks == 0) return 0;                        // one CTA per unit and no weights: nothing is left to do
-  return wide ? launch_after(kv_join_k<T, 1>, (unsigned)blocks, JT, st, a, (int)row_blocks)
-              : launch_after(kv_join_k<T, JT / 32>, (unsigned)blocks, JT, st, a, (int)row_blocks);
+  return wide ? launch_after(kv_join_k<T, 1, PER>, (unsigned)blocks, JT, st, a, (int)row_blocks)
+              : launch_after(kv_join_k<T, JT / 32, PER>, (unsigned)blocks, JT, st, a, (int)row_blocks);
+}
+template <typename T>
+int join(const KvAttnArgs& a, cudaStream_t st) {
+  return slots_of(a.T * a.group) == 8 ? join_rows<T, 8>(a, st) : join_rows<T, 4>(a, st);
 }
 
 }  // namespace kv
@@ -543,8 +565,8 @@ void kv_attn_plan(KvAttnArgs& a, int dtype, int sms) {
   a.nrb = (R + a.rows - 1) / a.rows;
   a.tile = a.hd <= 64 ? slab_keys<64>() : a.hd <= 128 ? slab_keys<128>() : slab_keys<256>();
   a.min_per = SW;
-  a.whole = 0;
-  a.extra = SW;
+  a.whole = a.S + a.T <= 4 * a.tile * SW;
+  a.extra = 10;
   a.ctas = (a.hd > 256 ? 1 : 2) * sms;
   bool vec = dtype == 0 && a.hd % 4 == 0;
   for (long s : {a.kn_b, a.kn_t, a.kn_h, a.vn_b, a.vn_t, a.vn_h, a.kc_b, a.kc_h, a.kc_s, a.vc_b, a.vc_h, a.vc_s}) vec = vec && s % 4 == 0;

@@ -496,8 +496,8 @@ void kv_attn_tc_plan(KvAttnArgs& a, int sms) {
   a.tile = SLAB * wr / ((a.hd > 64 ? 128 : 64) * 4);
   a.ctas = (wr == WARPS ? per_sm<WARPS>() : per_sm<1>()) * sms;
   a.min_per = WARPS / wr;
-  a.whole = 0;
-  a.extra = 3;
+  a.whole = a.S + a.T <= 4 * a.tile * WARPS / wr;
+  a.extra = a.rows <= 16 ? 8 : 4;
 }
 
 int kv_attn_tc_launch(const KvAttnArgs& a, int dtype, cudaStream_t st) {

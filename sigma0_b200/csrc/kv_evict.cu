@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(256) evict_move_k(KvEvictArgs a, int parts) {
   move_rows(a, a.moves + u * a.keep, u, a.count[u], (int)(blockIdx.x % parts) * 256 + threadIdx.x, 256 * parts);
 }
 
-constexpr int CT = 512, CMAX = 1024;
+constexpr int CT = 256, CMAX = 1024;
 
 template <typename V>
 __global__ void __launch_bounds__(CT) commit_k(KvCommitArgs a) {

@@ -76,23 +76,18 @@ def cache_evict(k_cache, v_cache, weight, positions, lengths, seen, keep, recent
     end move into free slots before it, in place.  A sequence of at most ``keep`` tokens stays as it is.
     Slots from the new length on get weight 0 and position -1.  ``out``: three tensors for the results,
     which may be the inputs themselves."""
-    kc, vc, w, p = (x if x.dim() > n else x.unsqueeze(0) for x, n in
-                    ((k_cache, 4), (v_cache, 4), (weight, 3), (positions, 3)))
-    ow, op, ol = out if out is not None else (None, None, None)
-    if out is not None and ow.dim() == 3:
-        ow, op = ow.unsqueeze(0), op.unsqueeze(0)
     if k_cache.is_cuda:
-        ow, op, ol = ext().kv_evict(kc, vc, w, p, lengths, seen, int(keep), int(recent), int(sinks), ow, op, ol)
-    else:
-        res = _evict_torch(kc, vc, w, p, lengths, seen, int(keep), int(recent), int(sinks))
-        if out is not None:
-            for o, r in zip((ow, op, ol), res):
-                o.copy_(r)
-        else:
-            ow, op, ol = res
-    if out is not None:
-        return tuple(out)
-    return (ow, op, ol) if weight.dim() == 4 else (ow[0], op[0], ol)
+        ow, op, ol = out if out is not None else (None, None, None)
+        return tuple(ext().kv_evict(k_cache, v_cache, weight, positions, lengths, seen, keep, recent, sinks, ow, op, ol))
+    layers = k_cache.dim() > 4
+    args = (k_cache, v_cache, weight, positions) if layers else (x.unsqueeze(0) for x in (k_cache, v_cache, weight, positions))
+    w, p, n = _evict_torch(*args, lengths, seen, keep, recent, sinks)
+    res = (w, p, n) if layers else (w[0], p[0], n)
+    if out is None:
+        return res
+    for o, r in zip(out, res):
+        o.copy_(r)
+    return tuple(out)
 
 
 def tree_commit(parents, tokens, targets, k_cache, v_cache, lengths, weight=None, positions=None, seen=None):
@@ -106,11 +101,12 @@ def tree_commit(parents, tokens, targets, k_cache, v_cache, lengths, weight=None
     ``lengths[b] + node``, move up to ``lengths[b] + 0, 1, ...`` in all layers; ``weight`` follows and is 0
     for the dropped ones, ``positions`` become ``seen[b] + 0, 1, ...`` and -1.  ``lengths`` and ``seen``
     stay as they are: add ``count`` to them."""
-    kc, vc = (x if x.dim() > 4 else x.unsqueeze(0) for x in (k_cache, v_cache))
-    w, p = (x if x is None or x.dim() > 3 else x.unsqueeze(0) for x in (weight, positions))
     if k_cache.is_cuda:
-        return tuple(ext().kv_commit(parents, tokens, targets, kc, vc, lengths, w, p, seen))
-    return _commit_torch(parents, tokens, targets, kc, vc, lengths, w, p, seen)
+        return tuple(ext().kv_commit(parents, tokens, targets, k_cache, v_cache, lengths, weight, positions, seen))
+    if k_cache.dim() == 4:
+        k_cache, v_cache = k_cache.unsqueeze(0), v_cache.unsqueeze(0)
+        weight, positions = (None if x is None else x.unsqueeze(0) for x in (weight, positions))
+    return _commit_torch(parents, tokens, targets, k_cache, v_cache, lengths, weight, positions, seen)
 
 
 # ---- torch expressions (CPU tensors) ------------------------------------------------------------
