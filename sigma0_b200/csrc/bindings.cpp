@@ -795,6 +795,14 @@ static void kv_caches(const at::Tensor& kc, const at::Tensor& vc, bool layers) {
   TORCH_CHECK(kc.size(-1) >= 1 && kc.size(-2) * kc.size(-1) < (int64_t)1 << 31, "a head's slots x channels must stay below 2^31");
 }
 
+// one word per device, like gemm_status
+at::Tensor kv_status(const at::Tensor& like) {
+  static std::vector<at::Tensor> per_dev(64);
+  const int d = like.device().index();
+  if (!per_dev[d].defined()) per_dev[d] = at::zeros({1}, like.options().dtype(at::kInt));
+  return per_dev[d];
+}
+
 at::Tensor kv_attn(at::Tensor q, at::Tensor kn, at::Tensor vn, at::Tensor kc, at::Tensor vc, at::Tensor lengths,
                    c10::optional<at::Tensor> mask, double scale, c10::optional<at::Tensor> weight,
                    c10::optional<at::Tensor> positions, c10::optional<at::Tensor> seen) {
@@ -853,6 +861,7 @@ at::Tensor kv_attn(at::Tensor q, at::Tensor kn, at::Tensor vn, at::Tensor kc, at
   a.B = (int)B; a.T = (int)T; a.nkv = (int)nkv; a.group = (int)(nh / nkv); a.hd = (int)hd; a.S = (int)S;
   a.scale_log2 = (float)(scale * 1.4426950408889634);
   a.inv_group = 1.f / (float)a.group;
+  a.status = kv_status(kc).data_ptr<int>();
   kv_attn_plan(a, dt, num_sms(kc));
   TORCH_CHECK(B * nh * T < (int64_t)1 << 30 && B * nkv * ((S + T) / 1024 + 1) < (int64_t)1 << 30, "too many heads and rows");
   const auto f32 = q.options().dtype(at::kFloat);
@@ -1636,6 +1645,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv_attn", &kv_attn, py::arg("q"), py::arg("k_new"), py::arg("v_new"), py::arg("k_cache"), py::arg("v_cache"),
         py::arg("lengths"), py::arg("mask"), py::arg("scale"), py::arg("weight"), py::arg("positions"), py::arg("seen"),
         "attention of T new tokens over a key / value cache that stores them (tree mask, accumulated weights)");
+  m.def("kv_status", [](at::Tensor like) { return kv_status(like); },
+        "status word of the tcgen05 cache attention (nonzero: a bounded wait ran out)");
   m.def("kv_evict", &kv_evict, py::arg("k_cache"), py::arg("v_cache"), py::arg("weight"), py::arg("positions"),
         py::arg("lengths"), py::arg("seen"), py::arg("keep"), py::arg("recent"), py::arg("sinks"),
         py::arg("weight_out"), py::arg("positions_out"), py::arg("lengths_out"),

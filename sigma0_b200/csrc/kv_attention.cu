@@ -556,8 +556,8 @@ int join(const KvAttnArgs& a, cudaStream_t st) {
 }  // namespace s0
 
 void kv_attn_plan(KvAttnArgs& a, int dtype, int sms) {
-  a.tc = kv_attn_tc_takes(a, dtype);
-  if (a.tc) return kv_attn_tc_plan(a, sms);
+  if (kv_attn_tc_takes(a, dtype)) return kv_attn_tc_plan(a, sms);
+  a.tc = 0;
   using namespace s0::kv;
   const int R = a.T * a.group;
   const int most = dtype ? 8 : a.hd <= 64 ? most_rows<64>() : a.hd <= 128 ? most_rows<128>() : most_rows<256>();

@@ -36,6 +36,22 @@ template <> struct Elem<__nv_bfloat16> {
   S0_DEV static __nv_bfloat16 of(float x) { return __float2bfloat16_rn(x); }
 };
 
+template <typename T> S0_DEV uint32_t pack2(float lo, float hi);
+template <> S0_DEV uint32_t pack2<__nv_bfloat16>(float lo, float hi) { return pack_bf16(lo, hi); }
+template <> S0_DEV uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// exponent bits all ones: infinity or NaN
+template <typename T> struct Inf;
+template <> struct Inf<__nv_bfloat16> { static constexpr uint32_t mask = 0x7f80u; };
+template <> struct Inf<__half> { static constexpr uint32_t mask = 0x7c00u; };
+template <typename T> S0_DEV bool any_inf(uint4 x) {
+  constexpr uint32_t m = Inf<T>::mask, hi = m << 16;
+  auto bad = [](uint32_t v) { return (v & m) == m || (v & hi) == hi; };
+  return bad(x.x) || bad(x.y) || bad(x.z) || bad(x.w);
+}
+
 // cached tokens of sequence b: a length outside [0, S] cannot be read or written past the cache
 S0_DEV int cached(const KvAttnArgs& a, int b) { return min(max(__ldg(a.lengths + b), 0), a.S); }
 

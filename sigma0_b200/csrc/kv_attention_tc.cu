@@ -1,9 +1,9 @@
 // Attention of a few new tokens over a 16-bit key / value cache on the tensor cores (the operator is
 // described in kv_attention.cu; heads up to 128 wide, 16-byte aligned rows).
 //
+// This kernel takes up to 16 rows (new tokens x query heads of a key head); more go to kv_attention_t5.cu.
 // What bounds it: a step reads every cached key and value once and does 4 T group flops per element
-// pair, so up to some 64 rows (new tokens x query heads of a key head) it is bound by HBM.  A CTA's
-// tiles (see kv_attention.cuh) form one stream, whose loads run ahead by cp.async across the ends of
+// pair: HBM.  A CTA's tiles (see kv_attention.cuh) form one stream, whose loads run ahead by cp.async across the ends of
 // units.
 //
 // The products are transposed: S^T = K Q^T and O^T = V^T P^T with mma.m16n8k16, so that the keys (then
@@ -12,10 +12,8 @@
 // fragment once for all its 8 NT rows, and the accumulators are half as large.  P^T comes out as
 // accumulators of the first product and goes into the second as its B operand; the two layouts are
 // transposes of one another, which movmatrix turns.
-//   NT  column groups of a warp: 8 or 16 rows;
-//   WR  warps that share a slab of keys for more rows: up to 64 rows in a CTA of four warps.
-// The other warps (4 / WR groups) take slabs of their own, each with a ring, a running maximum and a
-// running sum of its own and no barrier among groups; they are joined at the end of a unit.
+// NT: column groups, 8 rows each.  Every warp takes slabs of its own, with a ring, a running maximum and a
+// running sum of its own and no barrier among warps; they are joined at the end of a unit.
 //
 // The maximum that the exponentials refer to moves only when a score passes it by 2^8: the probabilities
 // may be up to 256 instead of 1, which changes no relative error, and the reduction over lanes and the
@@ -29,12 +27,6 @@
 namespace s0 {
 namespace kv {
 
-template <typename T> S0_DEV uint32_t pack2(float lo, float hi);
-template <> S0_DEV uint32_t pack2<__nv_bfloat16>(float lo, float hi) { return pack_bf16(lo, hi); }
-template <> S0_DEV uint32_t pack2<__half>(float lo, float hi) {
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
 template <typename T> S0_DEV void mma16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1);
 template <> S0_DEV void mma16<__nv_bfloat16>(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) { mma_bf16(c, a, b0, b1); }
 template <> S0_DEV void mma16<__half>(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -44,16 +36,6 @@ template <> S0_DEV void mma16<__half>(float* c, const uint32_t* a, uint32_t b0, 
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// exponent bits all ones: infinity or NaN
-template <typename T> struct Inf;
-template <> struct Inf<__nv_bfloat16> { static constexpr uint32_t mask = 0x7f80u; };
-template <> struct Inf<__half> { static constexpr uint32_t mask = 0x7c00u; };
-template <typename T> S0_DEV bool any_inf(uint4 x) {
-  constexpr uint32_t m = Inf<T>::mask, hi = m << 16;
-  auto bad = [](uint32_t v) { return (v & m) == m || (v & hi) == hi; };
-  return bad(x.x) || bad(x.y) || bad(x.z) || bad(x.w);
-}
-
 // byte offset of 16-byte chunk c of row r in a tile of HD 16-bit channels: the chunks of eight
 // consecutive rows fall into eight different groups of banks
 template <int HD> S0_DEV int tile_at(int r, int c) { return r * HD * 2 + ((c ^ (r & 7)) << 4); }
@@ -81,45 +63,32 @@ S0_DEV void put_slab(const char* st, const KvAttnArgs& a, int b, int h, int len,
       if (len + k0 + r < a.S) a.positions[b * a.pos_b + h * a.pos_h + len + k0 + r] = a.seen[b] + k0 + r;
 }
 
-constexpr int WARPS = 4, SLAB = 8192;   // warps, bytes of K and V per warp and stage
+constexpr int WARPS = 4, STAGES = 3, SLAB = 8192;   // warps, stages of a warp's ring, bytes of K and V in one
 
-// stages of a ring and CTAs of an SM: 64 rows are a longer chain of products per slab and want more warps,
-// fewer rows more bytes in flight per warp
-template <int WR> constexpr int stages() { return WR == WARPS ? 2 : 3; }
-template <int WR> constexpr int per_sm() { return WR == WARPS ? 3 : 2; }
-template <int HD, int WR> constexpr int slab_keys() { return SLAB * WR / (HD * 4); }
-// accumulators in passing: 2 warps (groups 2, 3 -> 0, 1) or WR warps (group 1 -> 0) at a time, maxima and sums
-template <int HD, int NT, int WR> constexpr int join_bytes() {
-  return WR == WARPS ? 0 : 2 * (HD / 16 * NT * 4 * 128 + NT * 8 * 2 * 4);
-}
+template <int HD> constexpr int slab_keys() { return SLAB / (HD * 4); }
+// two warps' accumulators, maxima and sums in passing
+template <int HD, int NT> constexpr int join_bytes() { return 2 * (HD / 16 * NT * 4 * 128 + NT * 8 * 2 * 4); }
 
-template <int N> S0_DEV void group_sync(int group) {
-  if constexpr (N == 1) __syncwarp();
-  else if constexpr (N == WARPS) __syncthreads();
-  else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(32 * N) : "memory");
-}
-
-template <typename T, int HD, int NT, int WR>
-__global__ void __launch_bounds__(32 * WARPS, per_sm<WR>()) kv_attn_tc_k(KvAttnArgs a, int ctas) {
-  constexpr int NK = slab_keys<HD, WR>(), WK = WARPS / WR, SB = SLAB * WR, NTH = 32 * WR, STAGES = stages<WR>();
+template <typename T, int HD, int NT>
+__global__ void __launch_bounds__(32 * WARPS, 2) kv_attn_tc_k(KvAttnArgs a, int ctas) {
+  constexpr int NK = slab_keys<HD>();
   constexpr int KG = NK % 32 == 0 ? 2 : 1;                      // groups of 16 keys in flight at once
-  constexpr int C = HD / 8, RS = NTH / C;                       // 16-byte chunks of a row, rows of a loading pass
+  constexpr int C = HD / 8, RS = 32 / C;                        // 16-byte chunks of a row, rows of a loading pass
   extern __shared__ __align__(128) char smem[];
   join_may_start();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int group = warp / WR, wr = warp % WR, gt = tid - group * NTH;
   const int R = a.T * a.group;
-  char* ring = smem + group * STAGES * SB;
-  float* sJ = reinterpret_cast<float*>(smem + WK * STAGES * SB);
+  char* ring = smem + warp * STAGES * SLAB;
+  float* sJ = reinterpret_cast<float*>(smem + WARPS * STAGES * SLAB);
   Cur cur;
   const long share = cta_share(cur, a, NK, reinterpret_cast<int*>(smem), ctas);
   __syncthreads();                                              // the plan's scratch becomes the rings
   if (share <= 0) return;
 
-  // ---- loading: this group's slabs of the share, ahead of their use -------------------------------
+  // ---- loading: this warp's slabs of the share, ahead of their use -------------------------------
   Cur ahead = cur;
-  int left = (int)((share - group + WK - 1) / WK);
-  const int ch = gt % C, lr = gt / C;                           // this thread's chunk and first row
+  int left = (int)((share - warp + WARPS - 1) / WARPS);
+  const int ch = lane % C, lr = lane / C;                           // this thread's chunk and first row
   const bool in = ch * 8 < a.hd;
   const char *kp = nullptr, *vp = nullptr;                      // its first row's addresses in the slab
   long ks = 0, vs = 0;                                          // bytes from pass to pass
@@ -140,20 +109,20 @@ __global__ void __launch_bounds__(32 * WARPS, per_sm<WR>()) kv_attn_tc_k(KvAttnA
   };
   auto fetch = [&](int stage) {
     if (left > 0) {
-      char* st = ring + stage * SB + tile_at<HD>(lr, ch);
+      char* st = ring + stage * SLAB + tile_at<HD>(lr, ch);
       const bool full = rows >= NK && a.hd == HD;
 #pragma unroll
       for (int i = 0; i < NK / RS; ++i) {
-        char* d = RS % 8 == 0 ? st + i * RS * HD * 2 : ring + stage * SB + tile_at<HD>(lr + i * RS, ch);
+        char* d = RS % 8 == 0 ? st + i * RS * HD * 2 : ring + stage * SLAB + tile_at<HD>(lr + i * RS, ch);
         const bool ok = full || (in && lr + i * RS < rows);
         cp_async16(d, ok ? kp + i * ks : (const char*)a.q, ok ? 16 : 0);
         cp_async16(d + NK * HD * 2, ok ? vp + i * vs : (const char*)a.q, ok ? 16 : 0);
       }
       if (--left > 0) {
-        if (cur_skip(ahead, a, NK, WK) && !fresh && rows > WK * NK) {
-          kp += ks * (WK * NK / RS);
-          vp += vs * (WK * NK / RS);
-          rows -= WK * NK;
+        if (cur_skip(ahead, a, NK, WARPS) && !fresh && rows > WARPS * NK) {
+          kp += ks * (WARPS * NK / RS);
+          vp += vs * (WARPS * NK / RS);
+          rows -= WARPS * NK;
         } else {
           aim();
         }
@@ -162,26 +131,26 @@ __global__ void __launch_bounds__(32 * WARPS, per_sm<WR>()) kv_attn_tc_k(KvAttnA
     cp_async_commit();
   };
   if (left > 0) {
-    cur_skip(ahead, a, NK, group);
+    cur_skip(ahead, a, NK, warp);
     aim();
   }
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) fetch(i);
 
   // ---- the units of the share ---------------------------------------------------------------------
-  long done = 0, mine = group;                                  // tiles before this unit, this group's next
+  long done = 0, mine = warp;                                   // tiles before this unit, this warp's next
   int stage = 0;
   while (done < share) {
-    const int b = cur.b, h = cur.u / a.nrb, rb = cur.u - h * a.nrb, r0 = rb * a.rows, row0 = r0 + wr * 8 * NT;
+    const int b = cur.b, h = cur.u / a.nrb, rb = cur.u - h * a.nrb, r0 = rb * a.rows;
     const long bh = (long)b * a.nkv + h;
     const int t1 = (int)min((long)cur.n, cur.t + (share - done));
     const int ncache = (cur.len + NK - 1) / NK;
     const long end = done + (t1 - cur.t);
-    // B fragments of Q^T: rows row0 + 8 nt + g
+    // B fragments of Q^T: rows r0 + 8 nt + g
     uint32_t qf[NT][HD / 16][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int row = row0 + 8 * nt + g, tok = div_group(a, row);
+      const int row = r0 + 8 * nt + g, tok = div_group(a, row);
       const T* p = (const T*)a.q + b * a.q_b + tok * a.q_t + (long)(h * a.group + row - tok * a.group) * a.q_h;
 #pragma unroll
       for (int k = 0; k < HD / 16; ++k)
@@ -203,12 +172,12 @@ __global__ void __launch_bounds__(32 * WARPS, per_sm<WR>()) kv_attn_tc_k(KvAttnA
       l[nt][0] = l[nt][1] = 0.f;                                // this lane's keys only, until the end
     }
 
-    for (; mine < end; mine += WK) {
+    for (; mine < end; mine += WARPS) {
       const int tt = cur.t + (int)(mine - done);
       cp_async_wait_group<STAGES - 2>();
-      group_sync<WR>(group);                                    // the slab is there, the one before it has been read
+      __syncwarp();                                             // the slab is there, the one before it has been read
       fetch(stage == 0 ? STAGES - 1 : stage - 1);
-      char* sk = ring + stage * SB;
+      char* sk = ring + stage * SLAB;
       char* sv = sk + NK * HD * 2;
       const bool tail = tt >= ncache;
       const int k0 = (tail ? tt - ncache : tt) * NK, nk = min(NK, (tail ? a.T : cur.len) - k0);
@@ -216,16 +185,16 @@ __global__ void __launch_bounds__(32 * WARPS, per_sm<WR>()) kv_attn_tc_k(KvAttnA
       // in V is taken out of the slab, and added by hand, after the product, to the rows that see it.
       bool bad = false;
       if (tail) {
-        if (rb == 0) put_slab<T, HD, NK>(sk, a, b, h, cur.len, k0, nk, gt, NTH);
+        if (rb == 0) put_slab<T, HD, NK>(sk, a, b, h, cur.len, k0, nk, lane, 32);
         for (int i = lane; i < NK * C; i += 32) bad |= any_inf<T>(*reinterpret_cast<const uint4*>(sv + i * 16));
         bad = __any_sync(0xffffffffu, bad);
         if (bad) {
-          group_sync<WR>(group);
-          for (int i = gt; i < NK * HD; i += NTH) {
+          __syncwarp();
+          for (int i = lane; i < NK * HD; i += 32) {
             unsigned short* p = reinterpret_cast<unsigned short*>(sv + tile_at<HD>(i / HD, (i % HD) >> 3) + (i & 7) * 2);
             if ((*p & Inf<T>::mask) == Inf<T>::mask) *p = 0;
           }
-          group_sync<WR>(group);
+          __syncwarp();
         }
       }
 #pragma unroll 1
@@ -251,7 +220,7 @@ __global__ void __launch_bounds__(32 * WARPS, per_sm<WR>()) kv_attn_tc_k(KvAttnA
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const int row = row0 + 8 * nt + 2 * t + e, tok = div_group(a, row);
+              const int row = r0 + 8 * nt + 2 * t + e, tok = div_group(a, row);
 #pragma unroll
               for (int q = 0; q < KG; ++q)
 #pragma unroll
@@ -268,7 +237,7 @@ __global__ void __launch_bounds__(32 * WARPS, per_sm<WR>()) kv_attn_tc_k(KvAttnA
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const int row = row0 + 8 * nt + 2 * t + e;
+              const int row = r0 + 8 * nt + 2 * t + e;
               if (row < R) {
                 float* p = a.scores + (bh * R + row) * a.sp + (tail ? cur.len : 0) + k0 + kk + g;
 #pragma unroll
@@ -344,7 +313,7 @@ __global__ void __launch_bounds__(32 * WARPS, per_sm<WR>()) kv_attn_tc_k(KvAttnA
           uint32_t vis = 0;
 #pragma unroll
           for (int i = 0; i < 2 * NT; ++i) {
-            const int row = row0 + (i >> 1) * 8 + 2 * t + (i & 1);
+            const int row = r0 + (i >> 1) * 8 + 2 * t + (i & 1);
             if (row < R && sees(a, b, div_group(a, row), k0 + j)) vis |= 1u << i;
           }
 #pragma unroll
@@ -369,67 +338,58 @@ __global__ void __launch_bounds__(32 * WARPS, per_sm<WR>()) kv_attn_tc_k(KvAttnA
         l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 16);
       }
 
-    // ---- join the groups: 2 and 3 hand over to 0 and 1, then 1 to 0 -------------------------------
-    if constexpr (WK > 1) {
-      constexpr int MT = HD / 16, PER = MT * NT * 4 * 32;
-      float* sM = sJ + 2 * PER;                                 // [2][8 NT][2]
-      auto give = [&](int slot) {
-        float* buf = sJ + slot * PER + lane;
-        float* ml = sM + slot * NT * 16 + 4 * t;                // rows 2 t, 2 t + 1 of a column group
+    // ---- join the warps: 2 and 3 hand over to 0 and 1, then 1 to 0 -------------------------------
+    constexpr int MT = HD / 16, PER = MT * NT * 4 * 32;
+    float* sM = sJ + 2 * PER;                                 // [2][8 NT][2]
+    auto give = [&](int slot) {
+      float* buf = sJ + slot * PER + lane;
+      float* ml = sM + slot * NT * 16 + 4 * t;                // rows 2 t, 2 t + 1 of a column group
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) buf[((i * NT + nt) * 4 + e) * 32] = o[i][nt][e];
-        if (g == 0) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            *reinterpret_cast<float4*>(ml + nt * 16) = make_float4(m[nt][0], l[nt][0], m[nt][1], l[nt][1]);
-        }
-      };
-      auto take = [&](int slot) {
-        const float* buf = sJ + slot * PER + lane;
-        const float* ml = sM + slot * NT * 16 + 4 * t;
+      for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float m2 = ml[nt * 16 + 2 * e], x = fmaxf(m[nt][e], m2);
-            const float e0 = x == -CUDART_INF_F ? 1.f : ex2(m[nt][e] - x), e1 = x == -CUDART_INF_F ? 0.f : ex2(m2 - x);
-            m[nt][e] = x;
-            l[nt][e] = l[nt][e] * e0 + ml[nt * 16 + 2 * e + 1] * e1;
+          for (int e = 0; e < 4; ++e) buf[((i * NT + nt) * 4 + e) * 32] = o[i][nt][e];
+      if (g == 0) {
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-              for (int y = 0; y < 2; ++y)
-                o[i][nt][2 * y + e] = o[i][nt][2 * y + e] * e0 + buf[((i * NT + nt) * 4 + 2 * y + e) * 32] * e1;
-          }
-      };
-      if constexpr (WK == 4) {
-        if (warp >= 2) give(warp - 2);
-        __syncthreads();
-        if (warp < 2) take(warp);
-        __syncwarp();
-        if (warp == 1) give(1);                                 // only this warp has read slot 1
-        __syncthreads();
-        if (warp == 0) take(1);
-        __syncthreads();                                        // the next unit may end at once for warp 3
-      } else {
-        if (group == 1) give(wr);
-        __syncthreads();
-        if (group == 0) take(wr);
-        __syncthreads();
+        for (int nt = 0; nt < NT; ++nt)
+          *reinterpret_cast<float4*>(ml + nt * 16) = make_float4(m[nt][0], l[nt][0], m[nt][1], l[nt][1]);
       }
-    }
-    if (group == 0) {
+    };
+    auto take = [&](int slot) {
+      const float* buf = sJ + slot * PER + lane;
+      const float* ml = sM + slot * NT * 16 + 4 * t;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float m2 = ml[nt * 16 + 2 * e], x = fmaxf(m[nt][e], m2);
+          const float e0 = x == -CUDART_INF_F ? 1.f : ex2(m[nt][e] - x), e1 = x == -CUDART_INF_F ? 0.f : ex2(m2 - x);
+          m[nt][e] = x;
+          l[nt][e] = l[nt][e] * e0 + ml[nt * 16 + 2 * e + 1] * e1;
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+              o[i][nt][2 * y + e] = o[i][nt][2 * y + e] * e0 + buf[((i * NT + nt) * 4 + 2 * y + e) * 32] * e1;
+        }
+    };
+    if (warp >= 2) give(warp - 2);
+    __syncthreads();
+    if (warp < 2) take(warp);
+    __syncwarp();
+    if (warp == 1) give(1);                                   // only this warp has read slot 1
+    __syncthreads();
+    if (warp == 0) take(1);
+    __syncthreads();                                          // the next unit may end at once for warp 3
+    if (warp == 0) {
       const bool first = cur.t == 0, all = first && t1 == cur.n;
       const long slot = 2L * blockIdx.x + (first ? 1 : 0);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int row = row0 + 8 * nt + 2 * t + e;
+          const int row = r0 + 8 * nt + 2 * t + e;
           if (row >= R) continue;
           if (all) {
             const int tok = div_group(a, row);
@@ -455,23 +415,17 @@ __global__ void __launch_bounds__(32 * WARPS, per_sm<WR>()) kv_attn_tc_k(KvAttnA
   }
 }
 
-template <typename T, int HD, int NT, int WR>
+template <typename T, int HD, int NT>
 int run_tc(const KvAttnArgs& a, cudaStream_t st) {
-  const size_t sm = std::max<size_t>(WARPS * stages<WR>() * SLAB + join_bytes<HD, NT, WR>(), (size_t)(a.B + 33) * 4);
-  const cudaError_t e = cudaFuncSetAttribute(kv_attn_tc_k<T, HD, NT, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
+  const size_t sm = std::max<size_t>(WARPS * STAGES * SLAB + join_bytes<HD, NT>(), (size_t)(a.B + 33) * 4);
+  const cudaError_t e = cudaFuncSetAttribute(kv_attn_tc_k<T, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
   if (e != cudaSuccess) return (int)e;
-  kv_attn_tc_k<T, HD, NT, WR><<<a.whole ? a.B * a.nkv * a.nrb : a.ctas, 32 * WARPS, sm, st>>>(a, a.ctas);
+  kv_attn_tc_k<T, HD, NT><<<a.whole ? a.B * a.nkv * a.nrb : a.ctas, 32 * WARPS, sm, st>>>(a, a.ctas);
   return (int)cudaGetLastError();
 }
-
 template <typename T, int HD>
 int launch_tc(const KvAttnArgs& a, cudaStream_t st) {
-  switch (a.rows) {
-    case 8: return run_tc<T, HD, 1, 1>(a, st);
-    case 16: return run_tc<T, HD, 2, 1>(a, st);
-    case 32: return run_tc<T, HD, 2, 2>(a, st);
-    default: return run_tc<T, HD, 2, 4>(a, st);
-  }
+  return a.rows == 8 ? run_tc<T, HD, 1>(a, st) : run_tc<T, HD, 2>(a, st);
 }
 
 }  // namespace kv
@@ -490,18 +444,20 @@ bool kv_attn_tc_takes(const KvAttnArgs& a, int dtype) {
 void kv_attn_tc_plan(KvAttnArgs& a, int sms) {
   using namespace s0::kv;
   const int R = a.T * a.group;
-  a.rows = R <= 8 ? 8 : R <= 16 ? 16 : R <= 32 ? 32 : 64;
-  a.nrb = (R + a.rows - 1) / a.rows;
-  const int wr = std::max(1, a.rows / 16);
-  a.tile = SLAB * wr / ((a.hd > 64 ? 128 : 64) * 4);
-  a.ctas = (wr == WARPS ? per_sm<WARPS>() : per_sm<1>()) * sms;
-  a.min_per = WARPS / wr;
-  a.whole = a.S + a.T <= 4 * a.tile * WARPS / wr;
-  a.extra = a.rows <= 16 ? 8 : 4;
+  if (R > 16) return kv_attn_t5_plan(a, sms);
+  a.tc = 1;
+  a.rows = R <= 8 ? 8 : 16;
+  a.nrb = 1;
+  a.tile = a.hd > 64 ? slab_keys<128>() : slab_keys<64>();
+  a.ctas = 2 * sms;
+  a.min_per = WARPS;
+  a.whole = a.S + a.T <= 4 * a.tile * WARPS;
+  a.extra = 8;
 }
 
 int kv_attn_tc_launch(const KvAttnArgs& a, int dtype, cudaStream_t st) {
   using namespace s0::kv;
+  if (a.tc == 2) return kv_attn_t5_launch(a, dtype, st);
   if (dtype == 1) return a.hd > 64 ? launch_tc<__half, 128>(a, st) : launch_tc<__half, 64>(a, st);
   return a.hd > 64 ? launch_tc<__nv_bfloat16, 128>(a, st) : launch_tc<__nv_bfloat16, 64>(a, st);
 }

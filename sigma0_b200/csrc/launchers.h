@@ -372,7 +372,7 @@ struct KvAttnArgs {
   int B, T, nkv, group, hd, S;
   float scale_log2;                   // softmax scale * log2(e)
   // set by kv_attn_plan: rows of a block, row blocks, keys of a tile, CTAs, least cost of a CTA, cost of a
-  // unit besides its tiles, one CTA per unit (no split), tensor cores, 16-byte loads of floats
+  // unit besides its tiles, one CTA per unit (no split), kernel (0 fp32, 1 mma.sync, 2 tcgen05), 16-byte loads of floats
   int rows, nrb, tile, ctas, min_per, extra, whole, tc, vec;
   // scratch: 2 * ctas pieces of [rows, hd] and [rows, 2]; with weights [B, nkv, T * group, sp] scores
   // and [B, nkv, T * group] log-sum-exps
@@ -380,9 +380,12 @@ struct KvAttnArgs {
   int* prefix;                        // [B + 1] tiles of one (head, row block) before every sequence
   long sp;
   float inv_group;                    // 1 / group
+  int* status;                        // set to 1 when a bounded wait of the tcgen05 kernel ran out
 };
 bool kv_attn_tc_takes(const KvAttnArgs& a, int dtype);
 void kv_attn_tc_plan(KvAttnArgs& a, int sms);
+void kv_attn_t5_plan(KvAttnArgs& a, int sms);
+int kv_attn_t5_launch(const KvAttnArgs& a, int dtype, cudaStream_t st);
 int kv_attn_tc_launch(const KvAttnArgs& a, int dtype, cudaStream_t st);
 void kv_attn_plan(KvAttnArgs& a, int dtype, int sms);
 int kv_attn_launch(const KvAttnArgs& a, int dtype, cudaStream_t st);
