@@ -9,7 +9,9 @@ Dense) -> residual``.  The attention projections keep Flax's
 FFN keeps ``ff/layers_0`` and ``ff/layers_2``.
 
 Decode uses a static KV cache ``(k (B,nh,max,hd), v, pos (B,))``; ``prefill``
-runs the training forward and fills the cache, like the reference.
+runs the training forward and fills the cache, like the reference.  ``decode`` runs over a
+cache of the caller's instead, with a length per sequence, a token budget and drafted trees
+(:mod:`sigma0_b200.ops.kv_cache`, :mod:`sigma0_b200.infer.speculative`).
 """
 from __future__ import annotations
 
@@ -170,3 +172,15 @@ class TransformerBlock(nn.Module):
         x = x + self.attn.out(o, self.compute_dtype).float()
         x = x + self.ff(self.norm2(x), self.compute_dtype).float()
         return (kc, vc, pos + L), x
+
+    def decode(self, x, attend, positions, mask=None):
+        """New tokens x (B, T, H) at absolute ``positions`` (B, T) over a cache of the caller's.
+
+        ``attend(q, k, v, mask)`` stores the new keys and values and returns the attention over the
+        cached and the new tokens (:meth:`sigma0_b200.ops.kv_cache.KVCache.attend`); ``mask`` says
+        which new tokens each of them sees (None: causal), so a tree of drafted tokens takes one pass."""
+        if self.use_pe:
+            x = x + sinusoidal_at(positions, x.shape[-1])
+        q, k, v = self._qkv(self.norm1(x))
+        x = x + self.attn.out(attend(q, k, v, mask), self.compute_dtype).float()
+        return x + self.ff(self.norm2(x), self.compute_dtype).float()

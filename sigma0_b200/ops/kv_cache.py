@@ -12,6 +12,7 @@ cache's shape without the head dimension, -1 in free slots) says which token a s
   and attends from them; ``lengths`` stays as it is until the caller adds the tokens that it keeps.
 * :func:`cache_evict` cuts every layer and head to ``keep`` tokens by accumulated weight.
 * :func:`tree_commit` accepts the longest path of a drafted tree that agrees with the model.
+* :class:`KVCache` holds the tensors of several layers and calls the three.
 
 CUDA tensors run the kernels of ``csrc/kv_attention.cu``, ``csrc/kv_attention_tc.cu`` and
 ``csrc/kv_evict.cu``; CPU tensors the torch expressions below.  Inference only: none of them has
@@ -107,6 +108,63 @@ def tree_commit(parents, tokens, targets, k_cache, v_cache, lengths, weight=None
         k_cache, v_cache = k_cache.unsqueeze(0), v_cache.unsqueeze(0)
         weight, positions = (None if x is None else x.unsqueeze(0) for x in (weight, positions))
     return _commit_torch(parents, tokens, targets, k_cache, v_cache, lengths, weight, positions, seen)
+
+
+class KVCache:
+    """The caches of several layers of one shape, with the lengths that they share.
+
+    ``k`` / ``v`` [layers, B, kv_heads, slots, head_dim]; with a ``budget`` every layer and head keeps at most
+    that many tokens (:meth:`trim`): the ``sinks`` first and ``recent`` last ones and those that received the most
+    attention.  All state changes in place, so a step over it can be captured in a CUDA graph."""
+
+    def __init__(self, layers, batch, kv_heads, slots, head_dim, dtype=torch.bfloat16, device=None, budget=None,
+                 recent=0, sinks=0):
+        if budget is not None and not 1 <= budget <= slots:
+            raise ValueError(f"a budget of 1 to {slots} tokens, got {budget}")
+        shape = (layers, batch, kv_heads, slots)
+        # zeros: a slot is read only once it holds a token, but a fresh cache should not look like data
+        self.k = torch.zeros(*shape, head_dim, dtype=dtype, device=device)
+        self.v = torch.zeros_like(self.k)
+        self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.seen = torch.zeros_like(self.lengths)
+        self.budget, self.recent, self.sinks = budget, recent, sinks
+        self.weight = self.positions = None
+        if budget is not None:
+            self.weight = torch.zeros(shape, dtype=torch.float32, device=device)
+            self.positions = torch.full(shape, -1, dtype=torch.int32, device=device)
+
+    @property
+    def slots(self):
+        return self.k.shape[3]
+
+    def attend(self, layer, q, k_new, v_new, mask=None, scale=None):
+        """:func:`cache_attention` of one layer; :meth:`add` or :meth:`commit` makes the tokens stay."""
+        w, p = (None, None) if self.weight is None else (self.weight[layer], self.positions[layer])
+        return cache_attention(q, k_new, v_new, self.k[layer], self.v[layer], self.lengths, mask=mask, scale=scale,
+                               weight=w, positions=p, seen=None if p is None else self.seen)
+
+    def add(self, n):
+        """The first ``n`` (an int, or int32 [B]) new tokens of the last step stay."""
+        self.lengths += n
+        self.seen += n
+
+    def commit(self, parents, tokens, targets):
+        """:func:`tree_commit` over all layers; the accepted tokens stay."""
+        path, count, token = tree_commit(parents, tokens, targets, self.k, self.v, self.lengths, weight=self.weight,
+                                         positions=self.positions, seen=self.seen if self.weight is not None else None)
+        self.add(count)
+        return path, count, token
+
+    def trim(self):
+        """:func:`cache_evict` to the budget, if there is one."""
+        if self.budget is not None:
+            cache_evict(self.k, self.v, self.weight, self.positions, self.lengths, self.seen, self.budget, self.recent,
+                        self.sinks, out=(self.weight, self.positions, self.lengths))
+
+
+def status(like: torch.Tensor) -> int:
+    """1 once a bounded wait of the tcgen05 attention gave up on this device (reads the device word)."""
+    return int(ext().kv_status(like).item())
 
 
 # ---- torch expressions (CPU tensors) ------------------------------------------------------------
