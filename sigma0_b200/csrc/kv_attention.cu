@@ -193,13 +193,13 @@ __global__ void __launch_bounds__(32 * SW, HDP == 512 ? 1 : 2) kv_attn_any_k(KvA
           }
         }
         bool far = false;
+        uint32_t see = kl < nk ? ~0u : 0u;
+        if (tail) see &= sees<RG>(a, b, k0 + kl, R, [=](int r) { return r0 + rg + r; });
 #pragma unroll
         for (int r = 0; r < RG; ++r) {
           if (DL > 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], 1);
           if (DL > 2) s[r] += __shfl_xor_sync(0xffffffffu, s[r], 2);
-          bool vis = kl < nk;
-          if (tail) vis &= (rg + r < nr) & sees(a, b, div_group(a, r0 + rg + r), k0 + kl);
-          if (!vis) s[r] = -CUDART_INF_F;
+          if (!(see >> r & 1)) s[r] = -CUDART_INF_F;
           if (a.scores && dl == 0 && kl < nk && rg + r < nr)
             a.scores[(bh * R + r0 + rg + r) * a.sp + (tail ? cur.len : 0) + k0 + kl] = s[r];
           far |= s[r] > __shfl_sync(0xffffffffu, m, rg + r) + 8.f;
@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(32 * SW, HDP == 512 ? 1 : 2) kv_attn_any_k(KvA
       if (bad) {
         const T* vn = (const T*)a.vn + b * a.vn_b + h * a.vn_h;
         for (int j = 0; j < nk; ++j) {
-          const unsigned vis = __ballot_sync(0xffffffffu, lane < nr && sees(a, b, div_group(a, r0 + lane), k0 + j));
+          const unsigned vis = __ballot_sync(0xffffffffu, lane < nr && sees<1>(a, b, k0 + j, R, [=](int) { return r0 + lane; }));
 #pragma unroll
           for (int c = 0; c < COLS; ++c) {
             const int d = COLS == 2 ? lane * 2 + c : lane * 4 + (c & 3) + (c >> 2) * 128;
@@ -415,17 +415,18 @@ __global__ void __launch_bounds__(JT) kv_join_k(KvAttnArgs a, int row_blocks) {
   const int b = (int)(bh / a.nkv), h = (int)(bh - (long)b * a.nkv);
   join_wait();
   Plan plan{0, 1};
-  int n = 1 + a.extra;                              // costs of a row block
+  int n = 1, surplus = 0;                           // costs of a row block, of them before its tiles
   long ub = 0;                                      // cost of the first tile of row block 0
   if (!a.whole) {
     plan = make_plan(a, a.prefix[a.B], a.ctas, a.min_per);
     const int p0 = a.prefix[b];
     n = a.prefix[b + 1] - p0;
-    ub = (long)p0 * a.nkv * a.nrb + (long)h * a.nrb * n + a.extra;
+    surplus = n - tiles_of(a, cached(a, b), a.tile);
+    ub = (long)p0 * a.nkv * a.nrb + (long)h * a.nrb * n + surplus;
   }
   auto pieces = [&](int rb) {
     const long s = ub + (long)rb * n;
-    return Pieces{s / plan.per, (s + n - a.extra - 1) / plan.per};
+    return Pieces{s / plan.per, (s + n - surplus - 1) / plan.per};
   };
   if (out) {
     const int row = (int)(min(idx, total - 1) - bh * R), rb = row / a.rows, r = row - rb * a.rows;
@@ -516,7 +517,7 @@ __global__ void __launch_bounds__(JT) kv_join_k(KvAttnArgs a, int row_blocks) {
 
 template <typename T, int HDP, int RB>
 int run_any(const KvAttnArgs& a, cudaStream_t st) {
-  const size_t sm = std::max(simt_bytes<HDP, RB>(), (size_t)(a.B + 33) * 4);
+  const size_t sm = std::max(simt_bytes<HDP, RB>(), (size_t)plan_ints(a.B) * 4);
   const cudaError_t e = cudaFuncSetAttribute(kv_attn_any_k<T, HDP, RB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
   if (e != cudaSuccess) return (int)e;
   kv_attn_any_k<T, HDP, RB><<<a.whole ? a.B * a.nkv * a.nrb : a.ctas, 32 * SW, sm, st>>>(a, a.ctas);
@@ -566,7 +567,8 @@ void kv_attn_plan(KvAttnArgs& a, int dtype, int sms) {
   a.tile = a.hd <= 64 ? slab_keys<64>() : a.hd <= 128 ? slab_keys<128>() : slab_keys<256>();
   a.min_per = SW;
   a.whole = a.S + a.T <= 4 * a.tile * SW;
-  a.extra = 10;
+  a.extra = 8;
+  a.least = 20;
   a.ctas = (a.hd > 256 ? 1 : 2) * sms;
   bool vec = dtype == 0 && a.hd % 4 == 0;
   for (long s : {a.kn_b, a.kn_t, a.kn_h, a.vn_b, a.vn_t, a.vn_h, a.kc_b, a.kc_h, a.kc_s, a.vc_b, a.vc_h, a.vc_s}) vec = vec && s % 4 == 0;

@@ -8,9 +8,11 @@
 // running maximum and sum), which a second kernel joins.  A CTA has at most two such pieces: the
 // end of one unit (slot 2 c) and the beginning of another (slot 2 c + 1).
 //
-// A unit costs something of its own (queries, the mask, the new rows, its output), which counts as
-// `a.extra` tiles at its beginning: the line is one of costs.  A CTA whose share begins within them
-// begins with tile 0, so tile t of a unit whose costs begin at s is CTA (s + extra + t) / per's.
+// A unit costs something of its own (queries, the mask, the new rows, its output), and the trips to
+// memory that a unit of few tiles takes are not covered by the streaming of its own tiles: it counts as
+// n tiles and `a.extra` more, `a.least` in all at least.  The line is one of these costs; the surplus lies
+// at the beginning of a unit, and a CTA whose share begins within it begins with tile 0, so tile t of a unit
+// whose costs begin at s is CTA (s + surplus + t) / per's.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -58,32 +60,54 @@ S0_DEV int cached(const KvAttnArgs& a, int b) { return min(max(__ldg(a.lengths +
 // key tiles of a sequence: its cached tokens, then the new ones (tiles never mix the two)
 S0_DEV int tiles_of(const KvAttnArgs& a, int len, int KT) { return (len + KT - 1) / KT + (a.T + KT - 1) / KT; }
 
-// s_pre[b] = costs of one (head, row block) before sequence b; returns the total.  Called by all
-// threads of the block; needs B + 1 + 32 ints of shared memory.
-S0_DEV long plan_prefix(const KvAttnArgs& a, int KT, int* s_pre) {
-  int* s_w = s_pre + a.B + 1;
+S0_DEV int cost_of(const KvAttnArgs& a, int tiles) { return max(tiles + a.extra, a.least); }
+
+// pre[b] = costs, pre[B + 1 + b] = tiles of one (head, row block) before sequence b; returns all costs.  Called
+// by all threads of the block; pre: plan_ints(B) of shared memory.
+__host__ __device__ constexpr int plan_ints(int B) { return 2 * (B + 1) + 64; }
+S0_DEV long plan_prefix(const KvAttnArgs& a, int KT, int* pre) {
+  int *s_w = pre + 2 * (a.B + 1), *tl = pre + a.B + 1;
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5;
   const int per = (a.B + nt - 1) / nt, b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
-  int sum = 0;
-  for (int b = b0; b < b1; ++b) sum += tiles_of(a, cached(a, b), KT) + a.extra;
-  int inc = sum;
+  int cost = 0, tiles = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int n = tiles_of(a, cached(a, b), KT);
+    cost += cost_of(a, n);
+    tiles += n;
+  }
+  int ic = cost, it = tiles;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += y;
+    const int x = __shfl_up_sync(0xffffffffu, ic, o), y = __shfl_up_sync(0xffffffffu, it, o);
+    if (lane >= o) {
+      ic += x;
+      it += y;
+    }
   }
-  if (lane == 31) s_w[warp] = inc;
+  if (lane == 31) {
+    s_w[warp] = ic;
+    s_w[32 + warp] = it;
+  }
   __syncthreads();
-  int base = 0;
-  for (int w = 0; w < warp; ++w) base += s_w[w];
-  int run = base + inc - sum;
+  ic -= cost;
+  it -= tiles;
+  for (int w = 0; w < warp; ++w) {
+    ic += s_w[w];
+    it += s_w[32 + w];
+  }
   for (int b = b0; b < b1; ++b) {
-    s_pre[b] = run;
-    run += tiles_of(a, cached(a, b), KT) + a.extra;
+    pre[b] = ic;
+    tl[b] = it;
+    const int n = tiles_of(a, cached(a, b), KT);
+    ic += cost_of(a, n);
+    it += n;
   }
-  if (b1 == a.B && b0 < a.B) s_pre[a.B] = run;
+  if (b1 == a.B && b0 < a.B) {
+    pre[a.B] = ic;
+    tl[a.B] = it;
+  }
   __syncthreads();
-  return s_pre[a.B];
+  return pre[a.B];
 }
 
 struct Plan {
@@ -100,12 +124,24 @@ S0_DEV Plan make_plan(const KvAttnArgs& a, long costs, int ctas, int min_per) {
 // row / group for rows below 2^20: (row + 1/2) / group is at least 1 / (2 group) away from an integer
 S0_DEV int div_group(const KvAttnArgs& a, int row) { return (int)((row + 0.5f) * a.inv_group); }
 
-// the mask row of new token t: which new tokens it sees
-// (indices past the new tokens are clamped, so that the loads need no branch and are in flight together)
-S0_DEV bool sees(const KvAttnArgs& a, int b, int t, int i) {
-  t = min(t, a.T - 1);
-  i = min(i, a.T - 1);
-  return a.mask ? a.mask[b * a.mask_b + (long)t * a.T + i] != 0 : i <= t;
+// Which of CNT rows (row(0), row(1), ...) see new token i, one bit each.  Indices past the end are clamped and
+// the choice between a mask and the causal order stands outside, so that the loads are in flight together.
+template <int CNT, typename F>
+S0_DEV uint32_t sees(const KvAttnArgs& a, int b, int i, int R, F row) {
+  uint32_t bits = 0;
+  const int j = min(i, a.T - 1);
+  if (a.mask) {
+    const unsigned char* m = a.mask + b * a.mask_b + j;
+    unsigned char x[CNT];
+#pragma unroll
+    for (int k = 0; k < CNT; ++k) x[k] = m[(long)min(div_group(a, row(k)), a.T - 1) * a.T];
+#pragma unroll
+    for (int k = 0; k < CNT; ++k) bits |= (uint32_t)((x[k] != 0) & (row(k) < R)) << k;
+  } else {
+#pragma unroll
+    for (int k = 0; k < CNT; ++k) bits |= (uint32_t)((j <= div_group(a, row(k))) & (row(k) < R)) << k;
+  }
+  return bits;
 }
 
 // 2^x: results below 2^-126 become 0
@@ -118,15 +154,17 @@ S0_DEV float ex2(float x) {
 // A unit and the place in it; steps from unit to unit in the plan's order.
 struct Cur {
   int b, u, len, n, t;  // sequence, head * nrb + row block, cached tokens, tiles, tile
+  int next;             // cached tokens of sequence b + 1: the trip for them is over before they are wanted
 };
-S0_DEV void cur_set(Cur& c, const KvAttnArgs& a, int KT) {
-  c.len = cached(a, c.b);
-  c.n = tiles_of(a, c.len, KT);
+S0_DEV void cur_set(Cur& c, const KvAttnArgs& a, int KT, int len) {
+  c.len = len;
+  c.n = tiles_of(a, len, KT);
+  c.next = c.b + 1 < a.B ? cached(a, c.b + 1) : 0;
 }
 S0_DEV void cur_next_unit(Cur& c, const KvAttnArgs& a, int KT) {
   if (++c.u == a.nkv * a.nrb) {
     c.u = 0;
-    if (++c.b < a.B) cur_set(c, a, KT);
+    if (++c.b < a.B) cur_set(c, a, KT, c.next);
   }
 }
 // true while the unit stays the same
@@ -141,7 +179,7 @@ S0_DEV bool cur_skip(Cur& c, const KvAttnArgs& a, int KT, int by) {
 }
 
 // The unit and tile at cost w of the line; returns how many tiles lie before it.
-S0_DEV long find_tile(Cur& c, const KvAttnArgs& a, const int* s_pre, long w) {
+S0_DEV long find_tile(Cur& c, const KvAttnArgs& a, const int* s_pre, long w, int KT) {
   const long hr = (long)a.nkv * a.nrb;
   int lo = 0, hi = a.B - 1;
   while (lo < hi) {  // the last b with pre[b] * hr <= w
@@ -151,12 +189,10 @@ S0_DEV long find_tile(Cur& c, const KvAttnArgs& a, const int* s_pre, long w) {
   const long rem = w - (long)s_pre[lo] * hr;
   const int cost = s_pre[lo + 1] - s_pre[lo];
   c.b = lo;
-  c.len = cached(a, lo);
-  c.n = cost - a.extra;
+  cur_set(c, a, KT, cached(a, lo));
   c.u = (int)(rem / cost);
-  const int x = (int)(rem - (long)c.u * cost);
-  c.t = max(0, x - a.extra);
-  return w - ((long)lo * hr + c.u) * a.extra - min(x, a.extra);
+  c.t = max(0, (int)(rem - (long)c.u * cost) - (cost - c.n));
+  return (long)s_pre[a.B + 1 + lo] * hr + (long)c.u * c.n + c.t;
 }
 
 // The first tile of this CTA and how many it has.  a.whole: one unit per CTA (caches that are short
@@ -167,7 +203,7 @@ S0_DEV long cta_share(Cur& c, const KvAttnArgs& a, int KT, int* scratch, int cta
     c.b = blockIdx.x / hr;
     c.u = blockIdx.x - c.b * hr;
     c.t = 0;
-    cur_set(c, a, KT);
+    cur_set(c, a, KT, cached(a, c.b));
     return c.n;
   }
   const Plan p = make_plan(a, plan_prefix(a, KT, scratch), ctas, a.min_per);
@@ -175,8 +211,8 @@ S0_DEV long cta_share(Cur& c, const KvAttnArgs& a, int KT, int* scratch, int cta
     for (int i = threadIdx.x; i <= a.B; i += blockDim.x) a.prefix[i] = scratch[i];
   const long w0 = (long)blockIdx.x * p.per, w1 = w0 + p.per;
   if (w0 >= p.total) return 0;
-  const long end = w1 < p.total ? find_tile(c, a, scratch, w1) : p.total - (long)a.B * hr * a.extra;
-  return end - find_tile(c, a, scratch, w0);
+  const long end = w1 < p.total ? find_tile(c, a, scratch, w1, KT) : (long)scratch[2 * a.B + 1] * hr;
+  return end - find_tile(c, a, scratch, w0, KT);
 }
 
 // Programmatic launch: the kernel behind this one may be set up while it runs, and waits for its results.

@@ -15,8 +15,9 @@
 // cp.async (rows past the end become 0, any strides), as far ahead as there are free slots.  Mbarriers
 // connect them; every wait is bounded: one that runs out sets a flag that ends all roles and a status word.
 //
-// A unit costs some 12 tiles besides its own (measured by sweeping `extra` on 16 ragged contexts of up to
-// 22,000 tokens, 64 nodes): the trips for queries, mask and new rows, and the output, which follow one another.
+// A unit costs some 8 tiles besides its own, and 20 at least (swept on 16 ragged contexts of up to 22,000 tokens
+// with 64 nodes: 529 us at 4 and 0, 385 us at 8 and 20): the trips for queries, mask bits and new rows take 3 us
+// each while the memory is busy, and only the tiles of a long unit cover them.
 //
 // The softmax's reference maximum moves only when a score passes it by 2^8 (see kv_attention_tc.cu); then
 // the rows' output in tensor memory is rescaled.  What bounds it: HBM up to 64 rows, if 64 columns x 128
@@ -43,13 +44,13 @@ template <int HD> struct Ring {
 };
 
 struct Bars {
-  uint64_t full[8], empty[8], sfull[2], sempty[2], qempty[2], pfull, pdone, mfull, mempty, drain;
+  uint64_t full[8], empty[8], sfull[2], sempty[2], qempty[2], pfull, pdone, mfull[2], mempty[2], drain;
   uint32_t tslot;
-  int abort;
+  int abort, bad[2];                                  // a wait ran out; a tile of new V is not finite
 };
 template <int HD> struct Smem {
   static constexpr int Q = Ring<HD>::SLOT * Ring<HD>::SLOTS, QB = N * 128 * (HD / 64), P = Q + 2 * QB, F = P + PANEL;
-  static constexpr int BYTES = F + (2 * N + 4 * N + 2 * KT) * 4 + (int)sizeof(Bars) + 1024;   // reference, factor, sums of 4 warps; mask bits
+  static constexpr int BYTES = F + (2 * N + 4 * N + 4 * KT) * 4 + (int)sizeof(Bars) + 1024;   // reference, factor, sums of 4 warps; mask bits
 };
 
 S0_DEV bool wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
@@ -117,8 +118,8 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
   float* s_m = reinterpret_cast<float*>(smem + SM::F);             // [N] references
   float* s_al = s_m + N;                                          // [N] factors, later 1 / sum
   float* s_l = s_al + N;                                          // [4][N] partial sums or maxima of the warps
-  uint32_t* s_vis = reinterpret_cast<uint32_t*>(s_l + 4 * N);      // [2][KT] rows that see a key, 32 bits each
-  Bars& bars = *reinterpret_cast<Bars*>(s_vis + 2 * KT);
+  uint32_t* s_vis = reinterpret_cast<uint32_t*>(s_l + 4 * N);      // [2][2][KT] rows that see a key, 32 bits each
+  Bars& bars = *reinterpret_cast<Bars*>(s_vis + 4 * KT);
   volatile int* abort = &bars.abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int R = a.T * a.group;
@@ -137,8 +138,10 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
     }
     tc::mbar_init(&bars.pfull, ST);
     tc::mbar_init(&bars.pdone, 1);
-    tc::mbar_init(&bars.mfull, 32);
-    tc::mbar_init(&bars.mempty, ST);
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&bars.mfull[i], 32);
+      tc::mbar_init(&bars.mempty[i], ST);
+    }
     tc::mbar_init(&bars.drain, 1);
     bars.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -158,46 +161,55 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
     for (int i = 0; i < share && ok;) {
       const int h = c.u / a.nrb, rb = c.u - h * a.nrb, r0 = rb * N, ncache = (c.len + KT - 1) / KT;
       const int t1 = min(c.n, c.t + (share - i)), from = max(c.t, ncache) - ncache;
+      const T *kn = (const T*)a.kn + c.b * a.kn_b + h * a.kn_h, *vn = (const T*)a.vn + c.b * a.vn_b + h * a.vn_h;
+      T* kc = (T*)a.kc + c.b * a.kc_b + h * a.kc_h + c.len * a.kc_s;
+      T* vc = (T*)a.vc + c.b * a.vc_b + h * a.vc_h + c.len * a.vc_s;
+      // rows [j0, j0 + n) of the new ones, behind the cached ones as far as they fit; true: one is not finite
+      auto copy = [&](const T* src, long ss, T* dst, long ds, int j0, int n, bool put) {
+        constexpr int C = HD / 8, RP = 32 / C, U = 16;             // chunks of a row, rows of a pass, passes in flight
+        const int ch = lane % C, fit = put ? a.S - c.len - j0 : 0;
+        bool bad = false;
+        src += (j0 + lane / C) * ss + ch * 8;
+        dst += (j0 + lane / C) * ds + ch * 8;
+        if (ch * 8 < a.hd)
+#pragma unroll 1
+          for (int j = lane / C; j < n; j += U * RP) {
+            uint4 x[U];
+#pragma unroll
+            for (int k = 0; k < U; ++k)
+              if (j + k * RP < n) x[k] = *reinterpret_cast<const uint4*>(src + k * RP * ss);
+#pragma unroll
+            for (int k = 0; k < U; ++k)
+              if (j + k * RP < n) {
+                bad |= any_inf<T>(x[k]);
+                if (j + k * RP < fit) *reinterpret_cast<uint4*>(dst + k * RP * ds) = x[k];
+              }
+            src += U * RP * ss;
+            dst += U * RP * ds;
+          }
+        __syncwarp();
+        return __any_sync(0xffffffffu, bad);
+      };
       for (int tt = from; tt < t1 - ncache; ++tt, ++tails) {
-        ok = wait(&bars.mempty, (tails & 1) ^ 1, abort);
+        const int j0 = tt * KT, n = min(KT, a.T - j0), buf = tails & 1;
+        ok = wait(&bars.mempty[buf], ((tails >> 1) & 1) ^ 1, abort);
         if (!ok) break;
 #pragma unroll 1
         for (int w = 0; w < 2 * KT / 32; ++w) {                    // 32 keys x 32 rows
-          const int k0 = tt * KT + (w & (KT / 32 - 1)) * 32, key = k0 + lane, q0 = r0 + w / (KT / 32) * 32;
+          const int k0 = j0 + (w & (KT / 32 - 1)) * 32, key = k0 + lane, q0 = r0 + w / (KT / 32) * 32;
           if (k0 >= a.T) continue;                                 // no such keys: nobody looks
-          uint32_t v = 0;
-          if (q0 < R)
-#pragma unroll
-          for (int x = 0; x < 32; ++x) v |= (uint32_t)((q0 + x < R) & sees(a, c.b, div_group(a, q0 + x), key)) << x;
-          s_vis[w * 32 + lane] = v;
+          const uint32_t v = q0 < R ? sees<32>(a, c.b, key, R, [=](int x) { return q0 + x; }) : 0u;
+          s_vis[(buf * 2 * KT) + w * 32 + lane] = v;
         }
-        tc::mbar_arrive(&bars.mfull);
-      }
-      if (rb == 0) {                                               // the rows go behind the cached ones
-        const int C = a.hd / 8, j0 = from * KT, n = (min(min(a.T, (t1 - ncache) * KT), a.S - c.len) - j0) * C;
-        const T *kn = (const T*)a.kn + c.b * a.kn_b + h * a.kn_h, *vn = (const T*)a.vn + c.b * a.vn_b + h * a.vn_h;
-        T* kc = (T*)a.kc + c.b * a.kc_b + h * a.kc_h + c.len * a.kc_s;
-        T* vc = (T*)a.vc + c.b * a.vc_b + h * a.vc_h + c.len * a.vc_s;
-        constexpr int U = 8;                                       // chunks in flight per lane
-        for (int e = lane; e < n; e += 32 * U) {
-          uint4 x[U], y[U];
-#pragma unroll
-          for (int k = 0; k < U; ++k)
-            if (e + 32 * k < n) {
-              const int j = j0 + (e + 32 * k) / C, d = (e + 32 * k) % C * 8;
-              x[k] = *reinterpret_cast<const uint4*>(kn + j * a.kn_t + d);
-              y[k] = *reinterpret_cast<const uint4*>(vn + j * a.vn_t + d);
-            }
-#pragma unroll
-          for (int k = 0; k < U; ++k)
-            if (e + 32 * k < n) {
-              const int j = j0 + (e + 32 * k) / C, d = (e + 32 * k) % C * 8;
-              *reinterpret_cast<uint4*>(kc + j * a.kc_s + d) = x[k];
-              *reinterpret_cast<uint4*>(vc + j * a.vc_s + d) = y[k];
-            }
+        const bool bad = copy(vn, a.vn_t, vc, a.vc_s, j0, n, rb == 0);
+        if (lane == 0) bars.bad[buf] = bad;
+        tc::mbar_arrive(&bars.mfull[buf]);
+        if (rb == 0) {
+          copy(kn, a.kn_t, kc, a.kc_s, j0, n, true);
+          if (a.positions)
+            for (int j = j0 + lane; j < min(j0 + n, a.S - c.len); j += 32)
+              a.positions[c.b * a.pos_b + h * a.pos_h + c.len + j] = a.seen[c.b] + j;
         }
-        if (a.positions)
-          for (int j = j0 + lane; j < j0 + n / C; j += 32) a.positions[c.b * a.pos_b + h * a.pos_h + c.len + j] = a.seen[c.b] + j;
       }
       i += t1 - c.t;
       c.t = 0;
@@ -327,6 +339,7 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
           break;
         }
         tc::fence_after_sync();
+        bool bad_tile = false;
         float s[W];
         tc::tmem_ld32(tmem + quad + (i & 1) * N, s);
         tc::fence_before_sync();
@@ -334,9 +347,11 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
         if (tail || nk < KT) {
           uint32_t vis = kt < nk ? ~0u : 0u;
           if (tail) {
-            dead |= !wait(&bars.mfull, tails & 1, abort);
-            vis &= s_vis[half * KT + kt];
-            tc::mbar_arrive(&bars.mempty);
+            const int buf = tails & 1;
+            dead |= !wait(&bars.mfull[buf], (tails >> 1) & 1, abort);
+            vis &= s_vis[buf * 2 * KT + half * KT + kt];
+            bad_tile = bars.bad[buf];
+            tc::mbar_arrive(&bars.mempty[buf]);
             ++tails;
           }
 #pragma unroll
@@ -399,21 +414,16 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
           *reinterpret_cast<uint4*>(sP + kt * 128 + (((half * (W / 8) + (c >> 3)) ^ (kt & 7)) << 4)) =
               make_uint4(pack2<T>(p[0], p[1]), pack2<T>(p[2], p[3]), pack2<T>(p[4], p[5]), pack2<T>(p[6], p[7]));
         }
-        if (tail && half) {
+        bad |= bad_tile;
+        if (bad_tile && half) {
           // what is not finite in V must not meet the zero probabilities of the rows that do not see it: it is
           // taken out of the tile here and added to the others' output at the end
           const int n = 2 * i + 1;
           dead |= !wait(&bars.full[n % SLOTS], (n / SLOTS) & 1, abort);
-          unsigned char* v = smem + (n % SLOTS) * RG::SLOT + kt * 128;
-#pragma unroll 2
-          for (int x = 0; x < HD / 8; ++x) {
-            uint4* at = reinterpret_cast<uint4*>(v + (x >> 3) * PANEL + ((x & 7) << 4));
-            if (any_inf<T>(*at)) {
-              bad = true;
-              unsigned short* e = reinterpret_cast<unsigned short*>(at);
-              for (int y = 0; y < 8; ++y)
-                if ((e[y] & Inf<T>::mask) == Inf<T>::mask) e[y] = 0;
-            }
+          unsigned short* v = reinterpret_cast<unsigned short*>(smem + (n % SLOTS) * RG::SLOT + kt * 128);
+          for (int x = 0; x < HD; ++x) {
+            unsigned short* e = v + (x >> 6) * (PANEL / 2) + (x & 63);
+            if ((*e & Inf<T>::mask) == Inf<T>::mask) *e = 0;
           }
         }
         tc::fence_proxy_async();
@@ -427,7 +437,6 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
       s_l[quarter * N + half * W + lane] = transpose_reduce<false>(l, lane);
       dead |= !wait(&bars.pdone, (i - 1) & 1, abort);
       if (any_of(dead)) break;
-      const bool add = any_of(bad);
       if (tid < N) {
         const float x = (s_l[tid] + s_l[N + tid]) + (s_l[2 * N + tid] + s_l[3 * N + tid]);
         const float m = s_m[tid] == UNSET ? -CUDART_INF_F : s_m[tid];
@@ -444,15 +453,16 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
       float o[W];
       tc::tmem_ld32(tmem + quad + TM_O, o);
       tc::fence_before_sync();
-      if (add && d < a.hd) {
+      if (bad && d < a.hd) {
         const T* vn = (const T*)a.vn + b * a.vn_b + h * a.vn_h + d;
         for (int j = 0; j < a.T; ++j) {
           const float x = Elem<T>::to(vn[j * a.vn_t]);
           const int tile = ncache + j / KT;
           if (isfinite(x) || tile < cur.t || tile >= t1) continue;
+          const uint32_t v = sees<W>(a, b, j, R, [=](int c) { return q0 + c; });
 #pragma unroll
           for (int c = 0; c < W; ++c)
-            if (q0 + c < R && sees(a, b, div_group(a, q0 + c), j)) o[c] += x;
+            if (v >> c & 1) o[c] += x;
         }
       }
       if (all) {
@@ -512,7 +522,8 @@ void kv_attn_t5_plan(KvAttnArgs& a, int sms) {
   a.ctas = sms;
   a.min_per = 1;
   a.whole = 0;
-  a.extra = 12;
+  a.extra = 8;
+  a.least = 20;
 }
 
 int kv_attn_t5_launch(const KvAttnArgs& a, int dtype, cudaStream_t st) {

@@ -217,19 +217,15 @@ __global__ void __launch_bounds__(32 * WARPS, 2) kv_attn_tc_k(KvAttnArgs a, int 
           }
         if (kk + 16 * KG > nk || tail) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int q = 0; q < KG; ++q)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int row = r0 + 8 * nt + 2 * t + e, tok = div_group(a, row);
+            for (int x = 0; x < 2; ++x) {
+              const int j = kk + 16 * q + g + 8 * x;
+              uint32_t vis = j < nk ? ~0u : 0u;
+              if (tail) vis &= sees<2 * NT>(a, b, k0 + j, R, [=](int i) { return r0 + (i >> 1) * 8 + 2 * t + (i & 1); });
 #pragma unroll
-              for (int q = 0; q < KG; ++q)
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                  const int j = kk + 16 * q + g + 8 * x;
-                  bool vis = j < nk;
-                  if (tail) vis &= (row < R) & sees(a, b, tok, k0 + j);
-                  if (!vis) s[q][nt][2 * x + e] = -CUDART_INF_F;
-                }
+              for (int i = 0; i < 2 * NT; ++i)
+                if (!(vis >> i & 1)) s[q][i >> 1][2 * x + (i & 1)] = -CUDART_INF_F;
             }
         }
         if (a.scores) {
@@ -310,12 +306,7 @@ __global__ void __launch_bounds__(32 * WARPS, 2) kv_attn_tc_k(KvAttnArgs a, int 
       if (bad) {
         const T* vn = (const T*)a.vn + b * a.vn_b + h * a.vn_h;
         for (int j = 0; j < nk; ++j) {
-          uint32_t vis = 0;
-#pragma unroll
-          for (int i = 0; i < 2 * NT; ++i) {
-            const int row = r0 + (i >> 1) * 8 + 2 * t + (i & 1);
-            if (row < R && sees(a, b, div_group(a, row), k0 + j)) vis |= 1u << i;
-          }
+          const uint32_t vis = sees<2 * NT>(a, b, k0 + j, R, [=](int i) { return r0 + (i >> 1) * 8 + 2 * t + (i & 1); });
 #pragma unroll
           for (int i = 0; i < HD / 8; ++i) {
             if (i * 8 >= a.hd) break;
@@ -417,7 +408,7 @@ __global__ void __launch_bounds__(32 * WARPS, 2) kv_attn_tc_k(KvAttnArgs a, int 
 
 template <typename T, int HD, int NT>
 int run_tc(const KvAttnArgs& a, cudaStream_t st) {
-  const size_t sm = std::max<size_t>(WARPS * STAGES * SLAB + join_bytes<HD, NT>(), (size_t)(a.B + 33) * 4);
+  const size_t sm = std::max<size_t>(WARPS * STAGES * SLAB + join_bytes<HD, NT>(), (size_t)plan_ints(a.B) * 4);
   const cudaError_t e = cudaFuncSetAttribute(kv_attn_tc_k<T, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
   if (e != cudaSuccess) return (int)e;
   kv_attn_tc_k<T, HD, NT><<<a.whole ? a.B * a.nkv * a.nrb : a.ctas, 32 * WARPS, sm, st>>>(a, a.ctas);
@@ -453,6 +444,7 @@ void kv_attn_tc_plan(KvAttnArgs& a, int sms) {
   a.min_per = WARPS;
   a.whole = a.S + a.T <= 4 * a.tile * WARPS;
   a.extra = 8;
+  a.least = 16;
 }
 
 int kv_attn_tc_launch(const KvAttnArgs& a, int dtype, cudaStream_t st) {

@@ -372,8 +372,8 @@ struct KvAttnArgs {
   int B, T, nkv, group, hd, S;
   float scale_log2;                   // softmax scale * log2(e)
   // set by kv_attn_plan: rows of a block, row blocks, keys of a tile, CTAs, least cost of a CTA, cost of a
-  // unit besides its tiles, one CTA per unit (no split), kernel (0 fp32, 1 mma.sync, 2 tcgen05), 16-byte loads of floats
-  int rows, nrb, tile, ctas, min_per, extra, whole, tc, vec;
+  // unit besides its tiles, its least cost, one CTA per unit (no split), kernel (0 fp32, 1 mma.sync, 2 tcgen05), 16-byte loads of floats
+  int rows, nrb, tile, ctas, min_per, extra, least, whole, tc, vec;
   // scratch: 2 * ctas pieces of [rows, hd] and [rows, 2]; with weights [B, nkv, T * group, sp] scores
   // and [B, nkv, T * group] log-sum-exps
   float *part_o, *part_ml, *scores, *lse;
