@@ -16,18 +16,26 @@
 namespace s0 {
 namespace kv {
 
-constexpr int SW = 4;  // warps of a block
+// warps of a block: wide heads leave one block on an SM
+template <int HDP> constexpr int simt_warps() { return HDP == 512 ? 8 : 4; }
 
-// Keys of a slab: one per lane (64 channels), or per 2 or 4 lanes that share its channels.  Its rows lie
+// two fp32 products and sums in one instruction
+S0_DEV unsigned long long fma2(unsigned long long x, unsigned long long y, unsigned long long z) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+  return r;
+}
+
+// Keys of a slab: one per lane (64 channels), or per 2, 4 or 8 lanes that share its channels.  Its rows lie
 // lane_parts * 4 words apart modulo 32 banks, so that the 8 lanes of a 16-byte access hit different banks.
-template <int HDP> constexpr int lane_parts() { return HDP == 64 ? 1 : HDP == 128 ? 2 : 4; }
+template <int HDP> constexpr int lane_parts() { return HDP / 64; }
 template <int HDP> constexpr int slab_keys() { return 32 / lane_parts<HDP>(); }
 template <int HDP> constexpr int slab_ld() { return HDP + 4 * lane_parts<HDP>(); }
 template <int HDP> constexpr int most_rows() { return HDP == 64 ? 32 : HDP == 128 ? 16 : 8; }
 template <int HDP, int RB> constexpr size_t simt_bytes() {
-  return 4 * ((size_t)SW * 2 * slab_keys<HDP>() * slab_ld<HDP>()   // K and V slabs
+  return 4 * ((size_t)simt_warps<HDP>() * 2 * slab_keys<HDP>() * slab_ld<HDP>()   // K and V slabs
               + RB * HDP                                          // queries
-              + SW * RB * (slab_keys<HDP>() + 4)                   // probabilities
+              + simt_warps<HDP>() * RB * (slab_keys<HDP>() + 4)                   // probabilities
               + 2 * RB * (HDP + 2));                               // two warps' results
 }
 
@@ -39,10 +47,11 @@ template <int HDP, int RB> constexpr size_t simt_bytes() {
 // probabilities as broadcasts.  K of the next slab is fetched while V is used and the other way round.
 // What bounds it: HBM for few rows (4 bytes per channel), the fp32 pipe from some 16 rows on.
 template <typename T, int HDP, int RB>
-__global__ void __launch_bounds__(32 * SW, HDP == 512 ? 1 : 2) kv_attn_any_k(KvAttnArgs a, int ctas) {
+__global__ void __launch_bounds__(32 * simt_warps<HDP>(), HDP == 512 ? 1 : 2) kv_attn_any_k(KvAttnArgs a, int ctas) {
+  constexpr int SW = simt_warps<HDP>();
   constexpr int DL = lane_parts<HDP>(), NK = slab_keys<HDP>(), LD = slab_ld<HDP>(), PL = NK + 4;
   constexpr int COLS = HDP / 32, RG = RB < 4 ? RB : 4;             // channels of a lane; rows at a time in the scores
-  constexpr int KQ = HDP / DL / 4, KH = KQ < 16 ? KQ : 16;         // 16-byte groups of a lane, of them in registers
+  constexpr int KH = HDP / DL / 4;                                 // 16-byte groups of channels of a lane
   constexpr int JS = COLS > 8 ? 2 : 4;                             // keys at a time in the output
   extern __shared__ __align__(16) float s_f[];
   join_may_start();
@@ -87,16 +96,22 @@ __global__ void __launch_bounds__(32 * SW, HDP == 512 ? 1 : 2) kv_attn_any_k(KvA
             for (int d = lane; d < a.hd; d += 32) cp_async4(dst + r * LD + d, r < rows ? src + r * rs + d : src, r < rows ? 4 : 0);
         }
       } else {
-        constexpr int U = 4;                                       // loads in flight per lane
-        for (int r = 0; r < NK; ++r)
-          for (int d0 = lane; d0 < a.hd; d0 += 32 * U) {
-            T x[U];
+        // element loads (odd alignments): 32 in flight per lane, or the slab waits for one trip after another
+        constexpr int CPL = HDP / 32, RU = 32 / CPL < NK ? 32 / CPL : NK;
+#pragma unroll 1
+        for (int r = 0; r < NK; r += RU) {
+          T x[RU][CPL];
 #pragma unroll
-            for (int k = 0; k < U; ++k) x[k] = r < rows && d0 + 32 * k < a.hd ? src[r * rs + d0 + 32 * k] : Elem<T>::of(0.f);
+          for (int y = 0; y < RU; ++y)
 #pragma unroll
-            for (int k = 0; k < U; ++k)
-              if (d0 + 32 * k < a.hd) dst[r * LD + d0 + 32 * k] = Elem<T>::to(x[k]);
-          }
+            for (int k = 0; k < CPL; ++k)
+              x[y][k] = r + y < rows && lane + 32 * k < a.hd ? src[(r + y) * rs + lane + 32 * k] : Elem<T>::of(0.f);
+#pragma unroll
+          for (int y = 0; y < RU; ++y)
+#pragma unroll
+            for (int k = 0; k < CPL; ++k)
+              if (lane + 32 * k < a.hd) dst[(r + y) * LD + lane + 32 * k] = Elem<T>::to(x[y][k]);
+        }
       }
       if (value && --left > 0) cur_skip(ahead, a, NK, SW);
     }
@@ -171,26 +186,20 @@ __global__ void __launch_bounds__(32 * SW, HDP == 512 ? 1 : 2) kv_attn_any_k(KvA
 #pragma unroll 1
       for (int rg = 0; rg < nr; rg += RG) {
         float s[RG];
+        ulonglong2 k[KH];                                        // two pairs of channels
 #pragma unroll
-        for (int r = 0; r < RG; ++r) s[r] = 0.f;
+        for (int i = 0; i < KH; ++i) k[i] = *reinterpret_cast<const ulonglong2*>(sK + kl * LD + (dl + DL * i) * 4);
 #pragma unroll
-        for (int half = 0; half < KQ / KH; ++half) {
-          float4 k[KH];
+        for (int r = 0; r < RG; ++r) {
+          unsigned long long x = 0, y = 0;
 #pragma unroll
-          for (int i = 0; i < KH; ++i) k[i] = *reinterpret_cast<const float4*>(sK + kl * LD + (dl + DL * (half * KH + i)) * 4);
-#pragma unroll
-          for (int r = 0; r < RG; ++r) {
-            float x = 0.f, y = 0.f;
-#pragma unroll
-            for (int i = 0; i < KH; ++i) {
-              const float4 q = *reinterpret_cast<const float4*>(sQ + (rg + r) * HDP + (dl + DL * (half * KH + i)) * 4);
-              x = fmaf(q.x, k[i].x, x);
-              y = fmaf(q.y, k[i].y, y);
-              x = fmaf(q.z, k[i].z, x);
-              y = fmaf(q.w, k[i].w, y);
-            }
-            s[r] += x + y;
+          for (int i = 0; i < KH; ++i) {
+            const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(sQ + (rg + r) * HDP + (dl + DL * i) * 4);
+            x = fma2(q.x, k[i].x, x);
+            y = fma2(q.y, k[i].y, y);
           }
+          const float2 u = *reinterpret_cast<const float2*>(&x), v = *reinterpret_cast<const float2*>(&y);
+          s[r] = (u.x + u.y) + (v.x + v.y);
         }
         bool far = false;
         uint32_t see = kl < nk ? ~0u : 0u;
@@ -199,6 +208,7 @@ __global__ void __launch_bounds__(32 * SW, HDP == 512 ? 1 : 2) kv_attn_any_k(KvA
         for (int r = 0; r < RG; ++r) {
           if (DL > 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], 1);
           if (DL > 2) s[r] += __shfl_xor_sync(0xffffffffu, s[r], 2);
+          if (DL > 4) s[r] += __shfl_xor_sync(0xffffffffu, s[r], 4);
           if (!(see >> r & 1)) s[r] = -CUDART_INF_F;
           if (a.scores && dl == 0 && kl < nk && rg + r < nr)
             a.scores[(bh * R + r0 + rg + r) * a.sp + (tail ? cur.len : 0) + k0 + kl] = s[r];
@@ -308,7 +318,7 @@ __global__ void __launch_bounds__(32 * SW, HDP == 512 ? 1 : 2) kv_attn_any_k(KvA
       fetch(sV, true);
     }
 
-    // ---- join the warps: 2 and 3 hand over to 0 and 1, then 1 to 0 --------------------------------
+    // ---- join the warps: the last two hand over to the two before, and so on; then 1 to 0 ----------
     auto give = [&](int slot) {
 #pragma unroll
       for (int r = 0; r < RB; ++r)
@@ -337,10 +347,14 @@ __global__ void __launch_bounds__(32 * SW, HDP == 512 ? 1 : 2) kv_attn_any_k(KvA
         for (int c = 0; c < COLS; ++c) o[r][c] = o[r][c] * f0 + sJ[((slot * RB + r) * COLS + c) * 32 + lane] * f1;
       }
     };
-    if (warp >= 2) give(warp - 2);
-    __syncthreads();
-    if (warp < 2) take(warp);
-    __syncwarp();
+#pragma unroll 1
+    for (int top = SW - 2; top >= 2; top -= 2) {
+      if (warp / 2 * 2 == top) give(warp & 1);
+      __syncthreads();
+      if (warp / 2 * 2 == top - 2) take(warp & 1);
+      __syncwarp();
+      if (top > 2) __syncthreads();
+    }
     if (warp == 1) give(1);                                        // only this warp has read slot 1
     __syncthreads();
     if (warp == 0) {
@@ -520,7 +534,7 @@ int run_any(const KvAttnArgs& a, cudaStream_t st) {
   const size_t sm = std::max(simt_bytes<HDP, RB>(), (size_t)plan_ints(a.B) * 4);
   const cudaError_t e = cudaFuncSetAttribute(kv_attn_any_k<T, HDP, RB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
   if (e != cudaSuccess) return (int)e;
-  kv_attn_any_k<T, HDP, RB><<<a.whole ? a.B * a.nkv * a.nrb : a.ctas, 32 * SW, sm, st>>>(a, a.ctas);
+  kv_attn_any_k<T, HDP, RB><<<a.whole ? a.B * a.nkv * a.nrb : a.ctas, 32 * simt_warps<HDP>(), sm, st>>>(a, a.ctas);
   return (int)cudaGetLastError();
 }
 template <typename T, int HDP>
@@ -564,9 +578,10 @@ void kv_attn_plan(KvAttnArgs& a, int dtype, int sms) {
   const int most = dtype ? 8 : a.hd <= 64 ? most_rows<64>() : a.hd <= 128 ? most_rows<128>() : most_rows<256>();
   a.rows = R == 1 ? 1 : R <= 8 ? 8 : most;
   a.nrb = (R + a.rows - 1) / a.rows;
-  a.tile = a.hd <= 64 ? slab_keys<64>() : a.hd <= 128 ? slab_keys<128>() : slab_keys<256>();
-  a.min_per = SW;
-  a.whole = a.S + a.T <= 4 * a.tile * SW;
+  a.tile = a.hd <= 64 ? slab_keys<64>() : a.hd <= 128 ? slab_keys<128>() : a.hd <= 256 ? slab_keys<256>() : slab_keys<512>();
+  const int warps = a.hd > 256 ? simt_warps<512>() : simt_warps<64>();
+  a.min_per = warps;
+  a.whole = a.S + a.T <= 4 * a.tile * warps;
   a.extra = 8;
   a.least = 20;
   a.ctas = (a.hd > 256 ? 1 : 2) * sms;

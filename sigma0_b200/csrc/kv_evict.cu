@@ -63,14 +63,13 @@ S0_DEV V block_scan(V v, V* s_w, V& total) {
 }
 
 // the rows of one unit's moves; V: the widest type that the rows' addresses and lengths are multiples of
-template <typename V>
+template <typename V, int U>             // U: pairs of rows in flight per thread
 S0_DEV void move_rows(const KvEvictArgs& a, const int2* mv, long u, int count, int i0, int step) {
   const int h = (int)(u % a.nkv), b = (int)(u / a.nkv % a.B), n = (int)(u / a.nkv / a.B);
   const unsigned C = a.hd * a.esize / (int)sizeof(V), total = count * C;
   char* kc = (char*)a.kc + (n * a.kc_n + b * a.kc_b + h * a.kc_h) * a.esize;
   char* vc = (char*)a.vc + (n * a.vc_n + b * a.vc_b + h * a.vc_h) * a.esize;
   const long ks = a.kc_s * a.esize, vs = a.vc_s * a.esize;
-  constexpr int U = 2;                   // pairs of rows in flight per thread
   for (unsigned i = i0; i < total; i += U * step) {
     V k[U], v[U];
     int to[U];
@@ -97,11 +96,12 @@ S0_DEV void move_rows(const KvEvictArgs& a, const int2* mv, long u, int count, i
     }
   }
 }
+template <int U>
 S0_DEV void move_rows(const KvEvictArgs& a, const int2* mv, long u, int count, int i0, int step) {
-  if (a.width == 16) move_rows<uint4>(a, mv, u, count, i0, step);
-  else if (a.width == 8) move_rows<uint2>(a, mv, u, count, i0, step);
-  else if (a.width == 4) move_rows<uint32_t>(a, mv, u, count, i0, step);
-  else move_rows<uint16_t>(a, mv, u, count, i0, step);
+  if (a.width == 16) move_rows<uint4, U>(a, mv, u, count, i0, step);
+  else if (a.width == 8) move_rows<uint2, U>(a, mv, u, count, i0, step);
+  else if (a.width == 4) move_rows<uint32_t, U>(a, mv, u, count, i0, step);
+  else move_rows<uint16_t, U>(a, mv, u, count, i0, step);
 }
 
 // The digit that holds the need-th largest value of a histogram: its bin, how many of it are needed.
@@ -125,7 +125,7 @@ S0_DEV void find_digit(const int* hist, int need, int* s_w, int* s_found) {
 
 // KEYS: all keys fit into shared memory
 template <int NT, bool KEYS>
-__global__ void __launch_bounds__(NT, 1536 / NT) evict_k(KvEvictArgs a, int moves_here) {
+__global__ void __launch_bounds__(NT, NT == 256 ? 8 : 1536 / NT) evict_k(KvEvictArgs a, int moves_here) {
   extern __shared__ __align__(16) uint32_t s_key[];    // [S], later the list of moves
   __shared__ int s_hist[EB], s_w[NT / 32 + 1], s_found[3];
   __shared__ unsigned long long s_w2[NT / 32 + 1];
@@ -242,7 +242,8 @@ __global__ void __launch_bounds__(NT, 1536 / NT) evict_k(KvEvictArgs a, int move
   }
   if (!moves_here) return;
   if (a.lengths_out != a.lengths && u < (long)a.B * a.nkv && h == 0 && tid == 0) a.lengths_out[b] = fin;
-  move_rows(a, list, u, moved, tid, NT);
+  // short units want more blocks on an SM (32 registers), long ones more rows in flight
+  move_rows<NT == 256 ? 1 : 2>(a, list, u, moved, tid, NT);
 }
 
 // the rows of all units, `parts` blocks each, and the new lengths; parts 0: the lengths only
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(256) evict_move_k(KvEvictArgs a, int parts) {
     for (int b = threadIdx.x; b < a.B; b += 256) a.lengths_out[b] = min(min(max(a.lengths[b], 0), a.S), a.keep);
   if (parts == 0) return;
   const long u = blockIdx.x / parts;
-  move_rows(a, a.moves + u * a.keep, u, a.count[u], (int)(blockIdx.x % parts) * 256 + threadIdx.x, 256 * parts);
+  move_rows<2>(a, a.moves + u * a.keep, u, a.count[u], (int)(blockIdx.x % parts) * 256 + threadIdx.x, 256 * parts);
 }
 
 constexpr int CT = 256, CMAX = 1024;
