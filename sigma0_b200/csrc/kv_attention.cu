@@ -19,6 +19,7 @@ namespace kv {
 // warps of a block: wide heads leave one block on an SM
 template <int HDP> constexpr int simt_warps() { return HDP == 512 ? 8 : 4; }
 
+S0_DEV void prefetch(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
 // two fp32 products and sums in one instruction
 S0_DEV unsigned long long fma2(unsigned long long x, unsigned long long y, unsigned long long z) {
   unsigned long long r;
@@ -45,7 +46,9 @@ template <int HDP, int RB> constexpr size_t simt_bytes() {
 // its key's channels in registers and reads the queries as broadcasts, 4 products per 16-byte load of
 // shared memory and row.  Output: a lane owns HDP / 32 channels of all rows, reads V once and the
 // probabilities as broadcasts.  K of the next slab is fetched while V is used and the other way round.
-// What bounds it: HBM for few rows (4 bytes per channel), the fp32 pipe from some 16 rows on.
+// What bounds it: HBM for few rows (one token, 8 contexts of up to 5,000, 16 x 128 floats: 86 us of a floor of 64), the
+// issue of fp32 products from some 16 rows on (22 rows over 8 contexts of up to 2,200, 16 x 64: 90 us of 15; 41% of the
+// issue slots at the two warps per scheduler that 250 registers leave).
 template <typename T, int HDP, int RB>
 __global__ void __launch_bounds__(32 * simt_warps<HDP>(), HDP == 512 ? 1 : 2) kv_attn_any_k(KvAttnArgs a, int ctas) {
   constexpr int SW = simt_warps<HDP>();
@@ -113,7 +116,18 @@ __global__ void __launch_bounds__(32 * simt_warps<HDP>(), HDP == 512 ? 1 : 2) kv
               if (lane + 32 * k < a.hd) dst[(r + y) * LD + lane + 32 * k] = Elem<T>::to(x[y][k]);
         }
       }
-      if (value && --left > 0) cur_skip(ahead, a, NK, SW);
+      if (value && --left > 0) {
+        cur_skip(ahead, a, NK, SW);
+        if constexpr (sizeof(T) == 2) {
+          // element loads are waited for: the lines of the slab after this one (32 of K, 32 of V) are on their way before
+          constexpr int LR = HDP / 64;                             // lines of a row
+          const int r = ahead.t * NK + lane / LR, at = lane % LR * 64, hh = ahead.u / a.nrb;
+          if (r < ahead.len && at < a.hd) {
+            prefetch((const T*)a.kc + ahead.b * a.kc_b + hh * a.kc_h + (long)r * a.kc_s + at);
+            prefetch((const T*)a.vc + ahead.b * a.vc_b + hh * a.vc_h + (long)r * a.vc_s + at);
+          }
+        }
+      }
     }
     cp_async_commit();
   };
@@ -388,7 +402,8 @@ __global__ void __launch_bounds__(32 * simt_warps<HDP>(), HDP == 512 ? 1 : 2) kv
   }
 }
 
-// Joins the pieces of the units that several CTAs share, and adds up the weights.  Blocks
+// Joins the pieces of the units that several CTAs share, and adds up the weights (64 books of up to
+// 11,000 slots, one row: 28 MB of scores and 56 MB of weights in 25-30 us, most of it latency).  Blocks
 // [0, row_blocks): rows of the output; the others: JT PER slots of one (sequence, key head) each.
 constexpr int JT = 256;
 // slots of a thread and rows at a time: one row wants many slots in flight, many rows share fewer
