@@ -15,6 +15,9 @@
 // NT: column groups, 8 rows each.  Every warp takes slabs of its own, with a ring, a running maximum and a
 // running sum of its own and no barrier among warps; they are joined at the end of a unit.
 //
+// Measured: one token of 64 books over up to 11,000 cached ones, 16 heads of 64: 290-300 us, 97% of the copy rate
+// (with queries as the 16-row side: 430 us); one token over 66,000, 16 heads of 128: 84-87 us, the copy rate.
+//
 // The maximum that the exponentials refer to moves only when a score passes it by 2^8: the probabilities
 // may be up to 256 instead of 1, which changes no relative error, and the reduction over lanes and the
 // rescaling of the output drop out of nearly every step.  p is rounded to the cache's type for the

