@@ -1,4 +1,4 @@
-// Shared parts of the cache kernels (kv_attention.cu, kv_attention_tc.cu, kv_evict.cu): how the
+// Shared parts of the cache kernels (kv_attention*.cu, kv_evict.cu): how the
 // keys of all sequences are split over the CTAs, and element types.
 //
 // The lengths live on the device, so the host cannot balance a ragged batch.  Every CTA derives

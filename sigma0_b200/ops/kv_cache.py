@@ -60,7 +60,8 @@ def cache_attention(q, k_new, v_new, k_cache, v_cache, lengths, mask=None, scale
     infinity in a token shows in no row that does not see it.  The new rows are stored in slots ``lengths[b] ...``; rows past the last slot are attended to but not stored.
 
     ``weight`` [B, kv_heads, slots] gets the probabilities of all T rows and of the group's query heads
-    added, ``positions`` the value ``seen[b] + i`` for new token i (both in place)."""
+    added (through a scratch of 4 bytes per row and slot), ``positions`` the value ``seen[b] + i`` for new
+    token i; both in place.  ``scale`` must be positive; k_new and v_new must not overlap the caches."""
     _inference_only(q, k_new, v_new, k_cache, v_cache)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if k_cache.is_cuda:
