@@ -44,6 +44,15 @@ template <> S0_DEV uint32_t pack2<__half>(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+// what two probabilities lose when they are packed, packed itself: the pair holds 16 (bf16) or 22 (fp16) bits of each
+template <typename T> S0_DEV uint32_t rest2(float lo, float hi, uint32_t packed);
+template <> S0_DEV uint32_t rest2<__nv_bfloat16>(float lo, float hi, uint32_t packed) {
+  return pack_bf16(lo - __uint_as_float(packed << 16), hi - __uint_as_float(packed & 0xffff0000u));
+}
+template <> S0_DEV uint32_t rest2<__half>(float lo, float hi, uint32_t packed) {
+  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&packed));
+  return pack2<__half>(lo - v.x, hi - v.y);
+}
 // exponent bits all ones: infinity or NaN
 template <typename T> struct Inf;
 template <> struct Inf<__nv_bfloat16> { static constexpr uint32_t mask = 0x7f80u; };
