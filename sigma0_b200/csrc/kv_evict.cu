@@ -17,9 +17,10 @@
 // with serial digit searches and a scan per 512 slots), bound by the selection: 53% of the issue slots and its barriers.
 //
 // Acceptance.  The walk down a tree of drafted tokens takes the lowest child whose token is the
-// model's token after the node, until there is none; row len + path[j] moves to len + j.  A child
-// has a higher index than its parent, so path[j] >= j and rows can move upwards in order.  64 nodes, 24 layers x 32 books: 16 us, a chain of four
-// trips to memory (tree, lengths, rows, weights); the rows themselves are 5 us.
+// model's token after the node, until there is none; row len + path[j] moves to len + j.  Nodes whose rows lie past
+// the last slot were not stored, and the walk does not go to them.  A child
+// has a higher index than its parent, so path[j] >= j and rows can move upwards in order.  64 nodes, 24 layers x 32 books: 14.5 us, a chain of three
+// trips to memory (tree and lengths, rows, weights); the rows themselves are 5 us.
 #include <algorithm>
 
 #include "kv_attention.cuh"
@@ -268,6 +269,7 @@ __global__ void __launch_bounds__(CT) commit_k(KvCommitArgs a) {
   __shared__ int s_cnt;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = blockIdx.x % a.B, n = blockIdx.x / a.B;
+  const int len = min(max(a.lengths[b], 0), a.S), fit = min(a.T, a.S - len);   // nodes whose rows are in the cache
   for (int i = tid; i < a.T; i += CT) {
     s_par[i] = a.parents[b * a.par_b + i];
     s_tok[i] = a.tokens[(long)b * a.T + i];
@@ -275,15 +277,15 @@ __global__ void __launch_bounds__(CT) commit_k(KvCommitArgs a) {
   }
   __syncthreads();
   if (warp == 0) {
-    int cur = 0, cnt = 1;
+    int cur = 0, cnt = fit > 0;
     if (lane == 0) s_path[0] = 0;
     while (true) {
       const long want = s_tgt[cur];
       int found = -1;
-      for (int i0 = (cur + 1) & ~31; i0 < a.T && found < 0; i0 += 32) {   // nodes above cur only: the walk ends
+      for (int i0 = (cur + 1) & ~31; i0 < fit && found < 0; i0 += 32) {   // nodes above cur only: the walk ends
         const int i = i0 + lane;
-        const bool fit = i > cur && i < a.T && s_par[i] == cur && s_tok[i] == want;
-        const unsigned any = __ballot_sync(0xffffffffu, fit);
+        const bool on = i > cur && i < fit && s_par[i] == cur && s_tok[i] == want;
+        const unsigned any = __ballot_sync(0xffffffffu, on);
         if (any) found = i0 + __ffs(any) - 1;
       }
       if (found < 0) break;
@@ -295,19 +297,18 @@ __global__ void __launch_bounds__(CT) commit_k(KvCommitArgs a) {
       s_cnt = cnt;
       if (n == 0) {
         a.count[b] = cnt;
-        a.next[b] = s_tgt[cur];
+        a.next[b] = cnt ? s_tgt[cur] : s_tok[0];
       }
     }
   }
   __syncthreads();
-  const int cnt = s_cnt, len = min(max(a.lengths[b], 0), a.S);
+  const int cnt = s_cnt;
   if (n == 0)
     for (int i = tid; i < a.T; i += CT) a.path[(long)b * a.T + i] = i < cnt ? s_path[i] : -1;
 
   // rows: a thread owns one column block of one head's K or V rows and moves them in order, eight loads
   // at a time (a destination never lies behind a later source)
   const int C = a.hd * a.esize / (int)sizeof(V);
-  const int fit = min(a.T, a.S - len);                   // new rows that are in the cache at all
   for (int i = tid; i < 2 * a.nkv * C; i += CT) {
     const int kv = i / (a.nkv * C), h = i / C % a.nkv;
     const long c = (long)(i % C) * sizeof(V);
@@ -319,10 +320,10 @@ __global__ void __launch_bounds__(CT) commit_k(KvCommitArgs a) {
       V x[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (j0 + j < cnt && s_path[j0 + j] < fit) x[j] = *reinterpret_cast<const V*>(base + s_path[j0 + j] * rs);
+        if (j0 + j < cnt) x[j] = *reinterpret_cast<const V*>(base + s_path[j0 + j] * rs);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (j0 + j < cnt && s_path[j0 + j] < fit) *reinterpret_cast<V*>(base + (j0 + j) * rs) = x[j];
+        if (j0 + j < cnt) *reinterpret_cast<V*>(base + (j0 + j) * rs) = x[j];
     }
   }
   for (int h = warp; h < a.nkv; h += CT / 32) {
@@ -330,7 +331,7 @@ __global__ void __launch_bounds__(CT) commit_k(KvCommitArgs a) {
     int* ps = a.positions ? a.positions + n * a.p_n + b * a.p_b + h * a.p_h + len : nullptr;
     for (int j0 = 0; j0 < fit; j0 += 32) {
       const int j = j0 + lane;
-      const bool on = j < cnt && j < fit && s_path[j] < fit;
+      const bool on = j < cnt;
       const float x = wt && on ? wt[s_path[j]] : 0.f;
       __syncwarp();
       if (j < fit) {

@@ -99,7 +99,8 @@ def tree_commit(parents, tokens, targets, k_cache, v_cache, lengths, weight=None
     or [B, T]), drafts ``tokens[b, i]`` (int64) and the model continues it with ``targets[b, i]``.  From the
     root the walk goes to the lowest child whose token is the model's, until there is none: ``path``
     int32 [B, T] holds its nodes (-1 behind them), ``count`` int32 [B] how many, ``token`` int64 [B] the
-    model's token after the last.  The path's rows, which :func:`cache_attention` left in slots
+    model's token after the last.  Nodes past the last slot have no rows and are not accepted; where not even
+    the root has one, ``count`` is 0 and ``token`` the root's own.  The path's rows, which :func:`cache_attention` left in slots
     ``lengths[b] + node``, move up to ``lengths[b] + 0, 1, ...`` in all layers; ``weight`` follows and is 0
     for the dropped ones, ``positions`` become ``seen[b] + 0, 1, ...`` and -1.  ``lengths`` and ``seen``
     stay as they are: add ``count`` to them."""
@@ -236,26 +237,25 @@ def _commit_torch(parents, tokens, targets, kc, vc, lengths, weight, positions, 
     count = torch.empty(B, dtype=torch.int32)
     token = torch.empty(B, dtype=torch.int64)
     for b in range(B):
-        walk = [0]
-        while True:
+        n = min(max(int(lengths[b]), 0), S)
+        fit = min(T, S - n)                                   # nodes whose rows are in the cache
+        walk = [0][:fit]
+        while walk:
             cur = walk[-1]
-            nxt = next((i for i in range(cur + 1, T) if par[b][i] == cur and tokens[b, i] == targets[b, cur]), None)
+            nxt = next((i for i in range(cur + 1, fit) if par[b][i] == cur and tokens[b, i] == targets[b, cur]), None)
             if nxt is None:
                 break
             walk.append(nxt)
-        n = min(max(int(lengths[b]), 0), S)
-        fit = min(T, S - n)
-        keep = [i for i in walk if i < fit]
-        rows = torch.tensor([n + i for i in keep], dtype=torch.long)
+        rows = torch.tensor([n + i for i in walk], dtype=torch.long)
         for cache in (kc, vc):
-            cache[:, b, :, n:n + len(keep)] = cache[:, b].index_select(2, rows)
+            cache[:, b, :, n:n + len(walk)] = cache[:, b].index_select(2, rows)
         if weight is not None:
             was = weight[:, b].index_select(2, rows)
             weight[:, b, :, n:n + fit] = 0.0
-            weight[:, b, :, n:n + len(keep)] = was
+            weight[:, b, :, n:n + len(walk)] = was
         if positions is not None:
             positions[:, b, :, n:n + fit] = -1
-            positions[:, b, :, n:n + len(keep)] = seen[b] + torch.arange(len(keep), dtype=torch.int32)
+            positions[:, b, :, n:n + len(walk)] = seen[b] + torch.arange(len(walk), dtype=torch.int32)
         path[b, :len(walk)] = torch.tensor(walk, dtype=torch.int32)
-        count[b], token[b] = len(walk), targets[b, walk[-1]]
+        count[b], token[b] = len(walk), targets[b, walk[-1]] if walk else tokens[b, 0]
     return path, count, token
