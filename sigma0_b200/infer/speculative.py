@@ -81,12 +81,26 @@ class TreeDecoder:
         for c in self.caches:
             c.trim()
 
-    def prefill(self, tokens, book=None, chunk=512):
-        """The prompt (B, L) in causal chunks that fit between budget and slots -> the model's next token (B,)."""
+    def _need(self, new, nodes=0):
+        """Raises where ``new`` tokens behind the cached ones do not fit, or a step of ``nodes`` beyond a budget that they reach."""
         c = self.caches[0]
+        rows = int(c.lengths.max()) + new
+        if c.budget:
+            rows = min(rows, c.budget + nodes)
+        if rows > c.slots:
+            raise ValueError(f"{rows} slots are needed, the caches have {c.slots}")
+
+    def prefill(self, tokens, book=None, chunk=512):
+        """The prompt (B, L) in causal chunks that fit between budget and slots -> the model's next token (B,).
+
+        Without a budget the prompt must fit behind the cached tokens (reads their number on the host)."""
+        c = self.caches[0]
+        if not tokens.shape[1]:
+            raise ValueError("a prompt of at least one token")
         chunk = min(chunk, 1024, c.slots - (c.budget or 0) if c.budget else c.slots)
         if chunk < 1:
             raise ValueError("no slots beyond the budget")
+        self._need(tokens.shape[1])
         for s in range(0, tokens.shape[1], chunk):
             part = tokens[:, s:s + chunk]
             rows = None if book is None else book if book.shape[1] == 1 else book[:, s:s + chunk]
@@ -123,10 +137,13 @@ def chain_tree(width, depth, device=None):
 def generate(decoder: TreeDecoder, prompt, n, book=None, width=2, depth=6, chunk=512):
     """Greedy tokens (B, n) after ``prompt`` (B, L) and the steps that they took.
 
-    ``book`` (B, 1, d_book): one row for all of the tokens.  ``depth`` 0: no drafts, one token a step."""
+    ``book`` (B, 1, d_book): one row for all of the tokens.  ``depth`` 0: no drafts, one token a step.  The caches
+    need a slot for each token of the prompt and of the result but the last, with a budget one for each of the
+    budget and of a step's 1 + width * depth nodes; ValueError where they have fewer."""
     B, L = prompt.shape
     dev = prompt.device
     nodes = 1 + width * depth
+    decoder._need(L + max(n, 1) - 1, nodes)
     history = torch.zeros(B, L + n + nodes, dtype=torch.long, device=dev)
     history[:, :L] = prompt
     length = torch.full((B,), L, dtype=torch.long, device=dev)
