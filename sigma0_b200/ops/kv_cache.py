@@ -131,6 +131,7 @@ class KVCache:
         self.seen = torch.zeros_like(self.lengths)
         self.budget, self.recent, self.sinks = budget, recent, sinks
         self.weight = self.positions = None
+        self._new = 0                                         # the most tokens of a step so far
         if budget is not None:
             self.weight = torch.zeros(shape, dtype=torch.float32, device=device)
             self.positions = torch.full(shape, -1, dtype=torch.int32, device=device)
@@ -142,19 +143,34 @@ class KVCache:
     def attend(self, layer, q, k_new, v_new, mask=None, scale=None):
         """:func:`cache_attention` of one layer; :meth:`add` or :meth:`commit` makes the tokens stay."""
         w, p = (None, None) if self.weight is None else (self.weight[layer], self.positions[layer])
+        self._new = max(self._new, q.shape[1])
         return cache_attention(q, k_new, v_new, self.k[layer], self.v[layer], self.lengths, mask=mask, scale=scale,
                                weight=w, positions=p, seen=None if p is None else self.seen)
 
     def add(self, n):
-        """The first ``n`` (an int, or int32 [B]) new tokens of the last step stay."""
-        self.lengths += n
+        """The first ``n`` (an int, or int32 [B]) new tokens of the last step stay; 0 takes the step back.
+
+        The others' slots are free again: their ``weight`` is 0 and their position -1.  What is past the last slot
+        was not stored and does not count in ``lengths``."""
+        self._keep(n)
+        if self.weight is not None and self._new and self.slots:
+            # the slots behind the new end that a step may have used; past the last one they name it again
+            at = (self.lengths.long()[:, None] + torch.arange(self._new, device=self.lengths.device))
+            free = at.clamp_max(self.slots - 1) >= self.lengths[:, None]
+            at = at.clamp_max(self.slots - 1)[:, None].expand(*self.weight.shape[:3], self._new)
+            free = free[:, None].expand_as(at)
+            self.weight.scatter_(-1, at, self.weight.gather(-1, at).masked_fill(free, 0.0))
+            self.positions.scatter_(-1, at, self.positions.gather(-1, at).masked_fill(free, -1))
+
+    def _keep(self, n):
+        self.lengths.add_(n).clamp_(max=self.slots)
         self.seen += n
 
     def commit(self, parents, tokens, targets):
         """:func:`tree_commit` over all layers; the accepted tokens stay."""
         path, count, token = tree_commit(parents, tokens, targets, self.k, self.v, self.lengths, weight=self.weight,
                                          positions=self.positions, seen=self.seen if self.weight is not None else None)
-        self.add(count)
+        self._keep(count)
         return path, count, token
 
     def trim(self):
