@@ -2,7 +2,7 @@
 // the acceptance of a drafted tree.
 //
 // Eviction.  Slot i of a unit (layer, sequence, key head) has the key
-//   top            if its position is among the first `sinks` or the last `recent` seen,
+//   top            if its position is among the first `sinks` or the last `recent` seen (-1, no position, is in neither),
 //   ord(weight_i)  otherwise (ord: unsigned integers in the order of the floats, NaN above all),
 // and the min(len, keep) largest stay, the lower slot first among equals.  The order of cached rows
 // means nothing to the attention, so only what lies behind the new end moves: the i-th survivor
@@ -32,7 +32,7 @@ constexpr int EB = 2048;                 // bins of a pass of 11 bits
 constexpr uint32_t HELD = 0xffffffffu;   // stays whatever its weight
 
 S0_DEV uint32_t order_key(float w, int pos, int seen, const KvEvictArgs& a) {
-  if (pos >= seen - a.recent || pos < a.sinks) return HELD;
+  if (pos >= 0 && (pos >= seen - a.recent || pos < a.sinks)) return HELD;
   if (w != w) return 0xfffffffeu;
   const uint32_t u = __float_as_uint(w + 0.f);  // -0 becomes 0
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);

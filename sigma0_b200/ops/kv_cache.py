@@ -73,7 +73,7 @@ def cache_evict(k_cache, v_cache, weight, positions, lengths, seen, keep, recent
     """Cut every sequence, layer and head to ``keep`` tokens -> (weight, positions, lengths).
 
     The tokens at positions below ``sinks`` and the ``recent`` last ones (positions from
-    ``seen[b] - recent``; ``seen[b]`` tokens have been through the sequence) stay, then those with the most
+    ``seen[b] - recent``; ``seen[b]`` tokens have been through the sequence; a token at -1 is neither) stay, then those with the most
     ``weight`` (the lower slot among equals; NaN counts as the most).  Rows of survivors behind the new
     end move into free slots before it, in place.  A sequence of at most ``keep`` tokens stays as it is.
     Slots from the new length on get weight 0 and position -1.  ``out``: three tensors for the results,
@@ -229,7 +229,7 @@ def _evict_torch(kc, vc, w, pos, lengths, seen, keep, recent, sinks):
     # float64 leaves room above every float32 weight for NaN and the held positions
     key = w.double().clamp(-1e300, 1e300)
     key = key.masked_fill(w.isnan(), 1e301)
-    key = key.masked_fill((pos >= seen[:, None, None] - recent) | (pos < sinks), 1e302)
+    key = key.masked_fill((pos >= 0) & ((pos >= seen[:, None, None] - recent) | (pos < sinks)), 1e302)
     order = key.masked_fill(slot >= ls, float("-inf")).sort(dim=-1, descending=True, stable=True).indices
     stays = torch.empty_like(order).scatter_(-1, order, slot.expand_as(order)) < new
     hole, mover = (slot < new) & ~stays, (slot >= new) & stays
