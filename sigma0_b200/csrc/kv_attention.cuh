@@ -53,6 +53,12 @@ template <> S0_DEV uint32_t rest2<__half>(float lo, float hi, uint32_t packed) {
   const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&packed));
   return pack2<__half>(lo - v.x, hi - v.y);
 }
+// The reference that the exponentials of a row refer to lies `up` below a maximum of its scores (base 2), and moves when a
+// score passes it by `far`.  Probabilities are then at most 2^far.  fp16 keeps nothing below 2^-25, which the many small
+// ones of a long context are beside one large one: with the reference 2^11 down that is 2^-36 of the largest.
+template <typename T> struct Ref;
+template <> struct Ref<__nv_bfloat16> { static constexpr float up = 0.f, far = 8.f; };
+template <> struct Ref<__half> { static constexpr float up = 11.f, far = 15.f; };
 // exponent bits all ones: infinity or NaN
 template <typename T> struct Inf;
 template <> struct Inf<__nv_bfloat16> { static constexpr uint32_t mask = 0x7f80u; };

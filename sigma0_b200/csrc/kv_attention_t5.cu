@@ -19,8 +19,10 @@
 // with 64 nodes: 529 us at 4 and 0, 385 us at 8 and 20): the trips for queries, mask bits and new rows take 3 us
 // each while the memory is busy, and only the tiles of a long unit cover them.
 //
-// The softmax's reference maximum moves only when a score passes it by 2^8 (see kv_attention_tc.cu); then
-// the rows' output in tensor memory is rescaled.  What bounds it: HBM up to 64 rows, if 64 columns x 128
+// The softmax's reference moves only when a score passes it by far (see kv_attention_tc.cu); then
+// the rows' output in tensor memory is rescaled.  p is rounded once to the cache's type for the second product: a second
+// tile for what that leaves does not fit beside the ring at 128 channels, and the error is 1.1 times that of the
+// output's own rounding (tree of 64 over 22,000 tokens).  What bounds it: HBM up to 64 rows, if 64 columns x 128
 // keys take less than the 64 KB of their K and V take from HBM (2,800 cycles of an SM at the copy rate):
 // the products read 6 KB of operands per 16-channel step from shared memory, some 770 cycles a tile; the
 // exponentials are 512 cycles of the SM's special function units.  Measured: 2,650-2,800 cycles a tile in a long unit;
@@ -366,7 +368,7 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
           for (int c = 0; c < W; ++c)
             if (q0 + c < R) p[c * a.sp] = s[c] * a.scale_log2;
         }
-        // does a score pass its row's reference by 2^8?
+        // does a score pass its row's reference?
         float over = -CUDART_INF_F;
 #pragma unroll
         for (int c = 0; c < W; c += 4) {
@@ -374,7 +376,7 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
           over = fmaxf(over, fmaxf(fmaxf(fmaf(s[c], a.scale_log2, -m.x), fmaf(s[c + 1], a.scale_log2, -m.y)),
                                    fmaxf(fmaf(s[c + 2], a.scale_log2, -m.z), fmaf(s[c + 3], a.scale_log2, -m.w))));
         }
-        const bool move = any_of(over > 8.f);
+        const bool move = any_of(over > Ref<T>::far);
         if (i > 0) dead |= !wait(&bars.pdone, (i - 1) & 1, abort);  // P and O^T of the tile before are done with
         if (move) {
           float x[W];
@@ -383,7 +385,7 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
           s_l[quarter * N + half * W + lane] = transpose_reduce<true>(x, lane);
           softmax_sync();
           if (tid < N) {
-            const float x = fmaxf(fmaxf(s_l[tid], s_l[N + tid]), fmaxf(s_l[2 * N + tid], s_l[3 * N + tid])) * a.scale_log2;
+            const float x = fmaxf(fmaxf(s_l[tid], s_l[N + tid]), fmaxf(s_l[2 * N + tid], s_l[3 * N + tid])) * a.scale_log2 - Ref<T>::up;
             const float was = s_m[tid], now = fmaxf(was, x);
             s_al[tid] = ex2(was - now);
             s_m[tid] = now;

@@ -18,9 +18,9 @@
 // Measured: one token of 64 books over up to 11,000 cached ones, 16 heads of 64: 290-300 us, 97% of the copy rate
 // (with queries as the 16-row side: 430 us); one token over 66,000, 16 heads of 128: 84-87 us, the copy rate.
 //
-// The maximum that the exponentials refer to moves only when a score passes it by 2^8: the probabilities
-// may be up to 256 instead of 1, which changes no relative error, and the reduction over lanes and the
-// rescaling of the output drop out of nearly every step.  p enters the second product as two numbers of the
+// The maximum that the exponentials refer to moves only when a score passes it by 2^8 (2^4 in fp16, whose range is
+// short: see Ref in kv_attention.cuh): the probabilities may be that much larger, which changes no relative error, and
+// the reduction over lanes and the rescaling of the output drop out of nearly every step.  p enters the second product as two numbers of the
 // cache's type, its rounding and what that left (16 bits of a bf16 p, 22 of an fp16 one): HBM hides the second
 // product (one token, 64 books: 322 us with and 319 us without it; 66,000 cached: 91.5 us both), and without it
 // the error of one token is 1.4 times the output's own rounding.  The sum of the row is taken from the
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(32 * WARPS, 2) kv_attn_tc_k(KvAttnArgs a, int 
               }
             }
         }
-        // does a score pass its row's reference by 2^8?
+        // does a score pass its row's reference?
         float mx[NT][2];
         bool far = false;
 #pragma unroll
@@ -260,14 +260,14 @@ __global__ void __launch_bounds__(32 * WARPS, 2) kv_attn_tc_k(KvAttnArgs a, int 
 #pragma unroll
             for (int q = 1; q < KG; ++q) x = fmaxf(x, fmaxf(s[q][nt][e], s[q][nt][2 + e]));
             mx[nt][e] = x * a.scale_log2;
-            far |= mx[nt][e] > m[nt][e] + 8.f;
+            far |= mx[nt][e] > m[nt][e] + Ref<T>::far;
           }
         if (__any_sync(0xffffffffu, far)) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float x = fmaxf(mx[nt][e], m[nt][e]);
+              float x = fmaxf(mx[nt][e] - Ref<T>::up, m[nt][e]);
               x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
               x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
               x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));

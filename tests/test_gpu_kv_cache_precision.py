@@ -1,4 +1,6 @@
 """What the cached attention of a 16-bit cache may lose: against 64-bit loops, next to the rounding of the output itself."""
+import math
+
 import pytest
 import torch
 
@@ -31,3 +33,34 @@ def test_up_to_16_rows_lose_the_output_rounding_only(B, T, nh, nkv, hd, S, lengt
     o64, _ = K.attention(q, kn, vn, kc, vc, lengths, None, hd ** -0.5)
     o = cache_attention(q, kn, vn, kc, vc, ls)
     assert K.rel(o, o64) < K.rel(o64.to(dtype), o64) + 2.0 ** -16 + 2.0 ** -12 * K.U[dtype]
+
+
+@pytest.mark.parametrize("dtype", [FH, BF])
+@pytest.mark.parametrize("T", [1, 12, 20])
+@pytest.mark.parametrize("drop", [19.0, 25.2, 27.5, 30.0])
+def test_one_dominant_token_beside_a_long_tail(T, drop, dtype):
+    """Keys with 2^-drop of the largest probability each, 20,000 of them, and a largest one whose value is 0: the output is the tail's.
+
+    The probabilities' absolute error is below 2^-36 of the largest each (fp16 keeps steps of 2^-24 and refers to 2^-11 of
+    the largest; a bf16 one has a relative error only), and the outputs are rounded, below 2^-14 in fp16 to steps of 2^-24."""
+    from sigma0_b200.ops.kv_cache import cache_attention
+    # as many units as CTAs and more: most are walked by one of them
+    B, nkv, hd, n = 2, 160, 64, 20000
+    S = n + T
+    kc = torch.zeros(B, nkv, S, hd, device="cuda", dtype=dtype)
+    vc, = _rand(T, (B, nkv, S, hd), dtype=dtype)
+    vc += 1
+    kc[:, :, (0, 32, 64, 96), 0] = drop          # one in each warp's first keys
+    vc[:, :, (0, 32, 64, 96)] = 0
+    q = torch.zeros(B, T, nkv, hd, device="cuda", dtype=dtype)
+    q[..., 0] = 8
+    kn = torch.zeros_like(q)
+    vn, = _rand(T + 1, q.shape, dtype=dtype)
+    scale = math.log(2) / 8                      # scores of `drop` and 0 in base 2
+    ls = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    o64, _ = K.attention(q, kn, vn, kc, vc, [n] * B, None, scale)
+    o = cache_attention(q, kn, vn, kc, vc, ls, scale=scale).double()
+    bound = 2 * K.U[dtype] * o64.abs()
+    if dtype == FH:
+        bound += 2.0 ** -25 + n * 2.0 ** -36 * 6  # |v| below 6
+    assert ((o - o64).norm(dim=-1) <= bound.norm(dim=-1)).all(), ((o - o64).norm() / bound.norm()).item()
