@@ -795,12 +795,14 @@ static void kv_caches(const at::Tensor& kc, const at::Tensor& vc, bool layers) {
   TORCH_CHECK(kc.size(-1) >= 1 && kc.size(-2) * kc.size(-1) < (int64_t)1 << 31, "a head's slots x channels must stay below 2^31");
 }
 
-// one word per device, like gemm_status
+// a variable of the kernel's module: there from its loading on, so a graph that is captured first neither owns nor clears it
 at::Tensor kv_status(const at::Tensor& like) {
-  static std::vector<at::Tensor> per_dev(64);
-  const int d = like.device().index();
-  if (!per_dev[d].defined()) per_dev[d] = at::zeros({1}, like.options().dtype(at::kInt));
-  return per_dev[d];
+  TORCH_CHECK(like.is_cuda(), "kv_status: a CUDA tensor");
+  c10::cuda::CUDAGuard guard(like.device());
+  int* word = nullptr;
+  const int rc = kv_status_word(&word);
+  TORCH_CHECK(rc == 0 && word, "kv_status failed (", str(rc), ")");
+  return at::from_blob(word, {1}, like.options().dtype(at::kInt));
 }
 
 at::Tensor kv_attn(at::Tensor q, at::Tensor kn, at::Tensor vn, at::Tensor kc, at::Tensor vc, at::Tensor lengths,
@@ -861,7 +863,6 @@ at::Tensor kv_attn(at::Tensor q, at::Tensor kn, at::Tensor vn, at::Tensor kc, at
   a.B = (int)B; a.T = (int)T; a.nkv = (int)nkv; a.group = (int)(nh / nkv); a.hd = (int)hd; a.S = (int)S;
   a.scale_log2 = (float)(scale * 1.4426950408889634);
   a.inv_group = 1.f / (float)a.group;
-  a.status = kv_status(kc).data_ptr<int>();
   kv_attn_plan(a, dt, num_sms(kc));
   TORCH_CHECK(B * nh * T < (int64_t)1 << 30 && B * nkv * ((S + T) / 1024 + 1) < (int64_t)1 << 30, "too many heads and rows");
   const auto f32 = q.options().dtype(at::kFloat);

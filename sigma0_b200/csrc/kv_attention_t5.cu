@@ -41,6 +41,7 @@ constexpr int KT = 128, N = 64, PANEL = KT * 128;     // keys of a tile, rows of
 constexpr int ST = 256, LT = 64, NT = ST + 32 + LT + 32;   // softmax threads, loading threads, threads
 constexpr int TM_O = 2 * N, TM_COLS = 256;            // tensor memory: S^T buffers at 0 and N, O^T
 constexpr unsigned long long WAIT_NS = 2000000000ull; // a wait that takes this long has failed
+__device__ int gave_up;                               // 1 once a wait has run out on this device
 constexpr float UNSET = -1e30f;                       // the reference of a row that has seen nothing
 
 template <int HD> struct Ring {
@@ -500,7 +501,7 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
   tc::fence_before_sync();
   __syncthreads();
   if (warp == ST / 32) tc::tmem_dealloc(tmem, TM_COLS);
-  if (tid == 0 && bars.abort) atomicExch(a.status, 1);
+  if (tid == 0 && bars.abort) atomicExch(&gave_up, 1);
 }
 
 template <typename T, int HD>
@@ -515,6 +516,8 @@ int run(const KvAttnArgs& a, cudaStream_t st) {
 }  // namespace t5
 }  // namespace kv
 }  // namespace s0
+
+int kv_status_word(int** word) { return (int)cudaGetSymbolAddress((void**)word, s0::kv::t5::gave_up); }
 
 // takes what kv_attn_tc_takes accepts
 void kv_attn_t5_plan(KvAttnArgs& a, int sms) {

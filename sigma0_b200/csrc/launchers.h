@@ -380,7 +380,6 @@ struct KvAttnArgs {
   int* prefix;                        // [B + 1] tiles of one (head, row block) before every sequence
   long sp;
   float inv_group;                    // 1 / group
-  int* status;                        // set to 1 when a bounded wait of the tcgen05 kernel ran out
 };
 bool kv_attn_tc_takes(const KvAttnArgs& a, int dtype);
 void kv_attn_tc_plan(KvAttnArgs& a, int sms);
@@ -389,6 +388,7 @@ int kv_attn_t5_launch(const KvAttnArgs& a, int dtype, cudaStream_t st);
 int kv_attn_tc_launch(const KvAttnArgs& a, int dtype, cudaStream_t st);
 void kv_attn_plan(KvAttnArgs& a, int dtype, int sms);
 int kv_attn_launch(const KvAttnArgs& a, int dtype, cudaStream_t st);
+int kv_status_word(int** word);        // the current device's word: 1 once a bounded wait of the tcgen05 kernel ran out
 
 // eviction from caches by accumulated weight (kv_evict.cu): N layers, B sequences, nkv heads
 struct KvEvictArgs {
