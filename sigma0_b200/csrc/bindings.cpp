@@ -6,6 +6,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <algorithm>
+#include <atomic>
 #include <cstdlib>
 #include <string>
 #include <vector>
@@ -805,6 +806,13 @@ at::Tensor kv_status(const at::Tensor& like) {
   return at::from_blob(word, {1}, like.options().dtype(at::kInt));
 }
 
+// bound of a wait of the tcgen05 kernel: far above any wait of a running one, also on a GPU that others share
+static std::atomic<uint64_t> kv_wait_ns{2000000000ull};
+void kv_wait_limit(double seconds) {
+  TORCH_CHECK(seconds >= 0 && seconds <= 60, "a limit of 0 to 60 seconds");
+  kv_wait_ns = (uint64_t)(seconds * 1e9);
+}
+
 at::Tensor kv_attn(at::Tensor q, at::Tensor kn, at::Tensor vn, at::Tensor kc, at::Tensor vc, at::Tensor lengths,
                    c10::optional<at::Tensor> mask, double scale, c10::optional<at::Tensor> weight,
                    c10::optional<at::Tensor> positions, c10::optional<at::Tensor> seen) {
@@ -863,6 +871,7 @@ at::Tensor kv_attn(at::Tensor q, at::Tensor kn, at::Tensor vn, at::Tensor kc, at
   a.B = (int)B; a.T = (int)T; a.nkv = (int)nkv; a.group = (int)(nh / nkv); a.hd = (int)hd; a.S = (int)S;
   a.scale_log2 = (float)(scale * 1.4426950408889634);
   a.inv_group = 1.f / (float)a.group;
+  a.wait_ns = kv_wait_ns;
   kv_attn_plan(a, dt, num_sms(kc));
   TORCH_CHECK(B * nh * T < (int64_t)1 << 30 && B * nkv * ((S + T) / 1024 + 1) < (int64_t)1 << 30, "too many heads and rows");
   const auto f32 = q.options().dtype(at::kFloat);
@@ -1648,6 +1657,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "attention of T new tokens over a key / value cache that stores them (tree mask, accumulated weights)");
   m.def("kv_status", [](at::Tensor like) { return kv_status(like); },
         "status word of the tcgen05 cache attention (nonzero: a bounded wait ran out)");
+  m.def("kv_wait_limit", &kv_wait_limit, py::arg("seconds"), "bound of the tcgen05 cache attention's waits");
   m.def("kv_evict", &kv_evict, py::arg("k_cache"), py::arg("v_cache"), py::arg("weight"), py::arg("positions"),
         py::arg("lengths"), py::arg("seen"), py::arg("keep"), py::arg("recent"), py::arg("sinks"),
         py::arg("weight_out"), py::arg("positions_out"), py::arg("lengths_out"),

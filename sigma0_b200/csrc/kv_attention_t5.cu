@@ -13,7 +13,7 @@
 // products, S of tile i + 1 before O of tile i; warp 11 stores the new rows and turns their mask into bits,
 // which takes several trips to a busy memory and nobody waits for; warps 9 and 10 load: K and V tiles go through a ring of slots by
 // cp.async (rows past the end become 0, any strides), as far ahead as there are free slots.  Mbarriers
-// connect them; every wait is bounded: one that runs out sets a flag that ends all roles and a status word.
+// connect them; every wait is bounded: one that runs out ends all roles, makes the CTA's rows NaN and sets a status word.
 //
 // A unit costs some 8 tiles besides its own, and 20 at least (swept on 16 ragged contexts of up to 22,000 tokens
 // with 64 nodes: 529 us at 4 and 0, 385 us at 8 and 20): the trips for queries, mask bits and new rows take 3 us
@@ -40,7 +40,7 @@ namespace t5 {
 constexpr int KT = 128, N = 64, PANEL = KT * 128;     // keys of a tile, rows of a unit, bytes of 64 channels of a tile
 constexpr int ST = 256, LT = 64, NT = ST + 32 + LT + 32;   // softmax threads, loading threads, threads
 constexpr int TM_O = 2 * N, TM_COLS = 256;            // tensor memory: S^T buffers at 0 and N, O^T
-constexpr unsigned long long WAIT_NS = 2000000000ull; // a wait that takes this long has failed
+constexpr unsigned long long DRAIN_NS = 2000000000ull;  // the bound of the wait for the last products, whatever the others' is
 __device__ int gave_up;                               // 1 once a wait has run out on this device
 constexpr float UNSET = -1e30f;                       // the reference of a row that has seen nothing
 
@@ -58,15 +58,16 @@ template <int HD> struct Smem {
   static constexpr int BYTES = F + (2 * N + 4 * N + 4 * KT) * 4 + (int)sizeof(Bars) + 1024;   // reference, factor, sums of 4 warps; mask bits
 };
 
-S0_DEV bool wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+// false: the wait took longer than `limit` ns, or another one has
+S0_DEV bool wait(uint64_t* bar, uint32_t parity, volatile int* abort, unsigned long long limit) {
   unsigned long long since = 0, now;
-  for (int i = 1;; ++i) {
+  for (int i = 1; limit; ++i) {
     if (tc::mbar_wait(bar, parity, 1)) return true;
     if (*abort) return false;
     if (i & 63) continue;
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
     if (since == 0) since = now;
-    if (now - since > WAIT_NS) break;
+    if (now - since > limit) break;
   }
   *abort = 1;
   return false;
@@ -197,7 +198,7 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
       };
       for (int tt = from; tt < t1 - ncache; ++tt, ++tails) {
         const int j0 = tt * KT, n = min(KT, a.T - j0), buf = tails & 1;
-        ok = wait(&bars.mempty[buf], ((tails >> 1) & 1) ^ 1, abort);
+        ok = __all_sync(0xffffffffu, wait(&bars.mempty[buf], ((tails >> 1) & 1) ^ 1, abort, a.wait_ns));   // the warp leaves as one
         if (!ok) break;
 #pragma unroll 1
         for (int w = 0; w < 2 * KT / 32; ++w) {                    // 32 keys x 32 rows
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
       const bool tail = c.t >= ncache;
       const int k0 = (tail ? c.t - ncache : c.t) * KT, rows = (tail ? a.T : c.len) - k0;
       if (fresh) {                                                 // a unit's queries come with its first keys
-        ok = wait(&bars.qempty[unit & 1], ((unit >> 1) & 1) ^ 1, abort);
+        ok = wait(&bars.qempty[unit & 1], ((unit >> 1) & 1) ^ 1, abort, a.wait_ns);
         if (!ok) break;
         for (int r = r0; r < N; r += RS) {
           const int row = rb * N + r, tok = div_group(a, row);
@@ -247,7 +248,7 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
       }
 #pragma unroll
       for (int v = 0; v < 2; ++v) {
-        ok = wait(&bars.empty[n % SLOTS], ((n / SLOTS) & 1) ^ 1, abort);
+        ok = wait(&bars.empty[n % SLOTS], ((n / SLOTS) & 1) ^ 1, abort, a.wait_ns);
         if (!ok) break;
         const long rs = v ? (tail ? a.vn_t : a.vc_s) : (tail ? a.kn_t : a.kc_s);
         const T* src = v ? (tail ? (const T*)a.vn + c.b * a.vn_b + h * a.vn_h : (const T*)a.vc + c.b * a.vc_b + h * a.vc_h)
@@ -279,7 +280,7 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
       for (int i = 0; i <= share && ok; ++i) {
         if (i < share) {                                           // S^T of tile i
           const int n = 2 * i;
-          ok = wait(&bars.full[n % SLOTS], (n / SLOTS) & 1, abort) && wait(&bars.sempty[i & 1], ((i >> 1) & 1) ^ 1, abort);
+          ok = wait(&bars.full[n % SLOTS], (n / SLOTS) & 1, abort, a.wait_ns) && wait(&bars.sempty[i & 1], ((i >> 1) & 1) ^ 1, abort, a.wait_ns);
           if (!ok) break;
           tc::fence_proxy_async();                                 // the loaders' copies, for the products
           tc::fence_after_sync();
@@ -292,7 +293,7 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
         }
         if (i > 0) {                                               // O^T of tile i - 1
           const int n = 2 * (i - 1) + 1;
-          ok = wait(&bars.pfull, (i - 1) & 1, abort) && wait(&bars.full[n % SLOTS], (n / SLOTS) & 1, abort);
+          ok = wait(&bars.pfull, (i - 1) & 1, abort, a.wait_ns) && wait(&bars.full[n % SLOTS], (n / SLOTS) & 1, abort, a.wait_ns);
           if (!ok) break;
           tc::fence_proxy_async();
           tc::fence_after_sync();
@@ -315,7 +316,7 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
       // nothing may be in flight when the tensor memory is given back
       tc::commit(&bars.drain);
       int none = 0;
-      wait(&bars.drain, 0, &none);
+      wait(&bars.drain, 0, &none, DRAIN_NS);
     }
     __syncwarp();
   } else {
@@ -338,7 +339,7 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
       for (int tt = cur.t; tt < t1; ++tt, ++i) {
         const bool tail = tt >= ncache;
         const int k0 = (tail ? tt - ncache : tt) * KT, nk = min(KT, (tail ? a.T : cur.len) - k0), key = k0 + kt;
-        dead |= !wait(&bars.sfull[i & 1], (i >> 1) & 1, abort);
+        dead |= !wait(&bars.sfull[i & 1], (i >> 1) & 1, abort, a.wait_ns);
         if (any_of(dead)) {
           stop = true;
           break;
@@ -353,7 +354,7 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
           uint32_t vis = kt < nk ? ~0u : 0u;
           if (tail) {
             const int buf = tails & 1;
-            dead |= !wait(&bars.mfull[buf], (tails >> 1) & 1, abort);
+            dead |= !wait(&bars.mfull[buf], (tails >> 1) & 1, abort, a.wait_ns);
             vis &= s_vis[buf * 2 * KT + half * KT + kt];
             bad_tile = bars.bad[buf];
             tc::mbar_arrive(&bars.mempty[buf]);
@@ -378,7 +379,7 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
                                    fmaxf(fmaf(s[c + 2], a.scale_log2, -m.z), fmaf(s[c + 3], a.scale_log2, -m.w))));
         }
         const bool move = any_of(over > Ref<T>::far);
-        if (i > 0) dead |= !wait(&bars.pdone, (i - 1) & 1, abort);  // P and O^T of the tile before are done with
+        if (i > 0) dead |= !wait(&bars.pdone, (i - 1) & 1, abort, a.wait_ns);  // P and O^T of the tile before are done with
         if (move) {
           float x[W];
 #pragma unroll
@@ -424,7 +425,7 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
           // what is not finite in V must not meet the zero probabilities of the rows that do not see it: it is
           // taken out of the tile here and added to the others' output at the end
           const int n = 2 * i + 1;
-          dead |= !wait(&bars.full[n % SLOTS], (n / SLOTS) & 1, abort);
+          dead |= !wait(&bars.full[n % SLOTS], (n / SLOTS) & 1, abort, a.wait_ns);
           unsigned short* v = reinterpret_cast<unsigned short*>(smem + (n % SLOTS) * RG::SLOT + kt * 128);
           for (int x = 0; x < HD; ++x) {
             unsigned short* e = v + (x >> 6) * (PANEL / 2) + (x & 63);
@@ -440,7 +441,7 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
       const bool first = cur.t == 0, all = first && t1 == cur.n;
       const long slot = 2L * blockIdx.x + (first ? 1 : 0);
       s_l[quarter * N + half * W + lane] = transpose_reduce<false>(l, lane);
-      dead |= !wait(&bars.pdone, (i - 1) & 1, abort);
+      dead |= !wait(&bars.pdone, (i - 1) & 1, abort, a.wait_ns);
       if (any_of(dead)) break;
       if (tid < N) {
         const float x = (s_l[tid] + s_l[N + tid]) + (s_l[2 * N + tid] + s_l[3 * N + tid]);
@@ -501,7 +502,29 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
   tc::fence_before_sync();
   __syncthreads();
   if (warp == ST / 32) tc::tmem_dealloc(tmem, TM_COLS);
-  if (tid == 0 && bars.abort) atomicExch(&gave_up, 1);
+  if (bars.abort) {                                                // all threads read the same: nobody writes it any more
+    // No output of this CTA can be told from memory that was never written: all of its rows become NaN, whole units
+    // here, pieces through their sums in the join.
+    if (tid == 0) atomicExch(&gave_up, 1);
+    const int tiles = (int)cta_share(cur, a, KT, reinterpret_cast<int*>(smem), ctas);
+    for (int i = 0; i < tiles;) {
+      const int h = cur.u / a.nrb, r0 = (cur.u - h * a.nrb) * N, nr = min(N, R - r0), t1 = min(cur.n, cur.t + (tiles - i));
+      if (cur.t == 0 && t1 == cur.n) {
+        for (int e = tid; e < nr * a.hd; e += NT) {
+          const int row = r0 + e / a.hd, tok = div_group(a, row);
+          ((T*)a.o)[(((long)cur.b * a.T + tok) * a.nkv * a.group + h * a.group + row - tok * a.group) * a.hd + e % a.hd] = Elem<T>::of(CUDART_NAN_F);
+        }
+        if (a.lse)
+          for (int r = tid; r < nr; r += NT) a.lse[((long)cur.b * a.nkv + h) * R + r0 + r] = CUDART_NAN_F;
+      } else {
+        for (int r = tid; r < nr; r += NT)
+          *reinterpret_cast<float2*>(a.part_ml + ((2L * blockIdx.x + (cur.t == 0 ? 1 : 0)) * a.rows + r) * 2) = make_float2(0.f, CUDART_NAN_F);
+      }
+      i += t1 - cur.t;
+      cur.t = 0;
+      cur_next_unit(cur, a, KT);
+    }
+  }
 }
 
 template <typename T, int HD>

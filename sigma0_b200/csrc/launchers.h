@@ -380,6 +380,7 @@ struct KvAttnArgs {
   int* prefix;                        // [B + 1] tiles of one (head, row block) before every sequence
   long sp;
   float inv_group;                    // 1 / group
+  unsigned long long wait_ns;         // bound of the tcgen05 kernel's waits
 };
 bool kv_attn_tc_takes(const KvAttnArgs& a, int dtype);
 void kv_attn_tc_plan(KvAttnArgs& a, int sms);

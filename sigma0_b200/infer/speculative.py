@@ -19,7 +19,7 @@ import time
 import torch
 
 from ..models.transformer import TransformerBlock
-from ..ops.kv_cache import KVCache, tree_depth, tree_mask
+from ..ops.kv_cache import KVCache, check, tree_depth, tree_mask
 
 
 class TreeDecoder:
@@ -139,7 +139,8 @@ def generate(decoder: TreeDecoder, prompt, n, book=None, width=2, depth=6, chunk
 
     ``book`` (B, 1, d_book): one row for all of the tokens.  ``depth`` 0: no drafts, one token a step.  The caches
     need a slot for each token of the prompt and of the result but the last, with a budget one for each of the
-    budget and of a step's 1 + width * depth nodes; ValueError where they have fewer."""
+    budget and of a step's 1 + width * depth nodes; ValueError where they have fewer.  RuntimeError if an attention
+    kernel gave up (:func:`sigma0_b200.ops.kv_cache.check`)."""
     B, L = prompt.shape
     dev = prompt.device
     nodes = 1 + width * depth
@@ -169,6 +170,7 @@ def generate(decoder: TreeDecoder, prompt, n, book=None, width=2, depth=6, chunk
         # sequences that are done keep going (their tokens are cut off) until the slowest is
         length = torch.minimum(length + count, torch.full_like(length, history.shape[1] - nodes))
         steps += 1
+    check(history)
     return history[:, L:L + n], steps
 
 

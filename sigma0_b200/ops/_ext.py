@@ -14,7 +14,7 @@ _C = None
 _COUNT = [0]
 # kernels launched per call, where it is not one
 _LAUNCHES = {"m3_fwd": 2, "m3_bwd": 5, "ln_bwd": 2, "rms_bwd": 2, "glu_res_bwd": 2, "attn_bwd": 2, "s5_scan_fwd": 3, "s5_scan_bwd": 3,
-             "kv_attn": 2, "kv_evict": 2}
+             "kv_attn": 2, "kv_evict": 2, "kv_status": 0, "kv_wait_limit": 0}
 
 
 class _Counted:

@@ -185,6 +185,22 @@ def status(like: torch.Tensor) -> int:
     return int(ext().kv_status(like).item())
 
 
+def check(like: torch.Tensor) -> None:
+    """RuntimeError if :func:`status` is set, which is cleared then; reads the device word, so it waits for the stream.
+
+    The call whose wait gave up has NaN in the rows concerned and may not have stored its new tokens."""
+    if like.is_cuda and status(like):
+        ext().kv_status(like).zero_()
+        raise RuntimeError("cached attention: a wait inside a kernel took longer than its limit; the outputs since are not valid")
+
+
+def wait_limit(seconds: float = 2.0) -> None:
+    """How long a wait inside the tcgen05 attention may take (calls from now on; a captured call keeps its own).
+
+    At 0 every wait gives up at once, which shows what a caller does then."""
+    ext().kv_wait_limit(float(seconds))
+
+
 # ---- torch expressions (CPU tensors) ------------------------------------------------------------
 def _attention_torch(q, k_new, v_new, kc, vc, lengths, mask, scale, weight, positions, seen):
     B, T, nh, hd = q.shape
