@@ -878,13 +878,13 @@ at::Tensor kv_attn(at::Tensor q, at::Tensor kn, at::Tensor vn, at::Tensor kc, at
   // one scratch tensor: pieces [2 ctas, rows, hd + 2], then with weights the scores and row sums
   const int64_t po = 2LL * a.ctas * a.rows * hd, ml = 4LL * a.ctas * a.rows, R = T * (nh / nkv);
   a.sp = (S + T + 3) / 4 * 4;
-  const int64_t sc = a.weight ? B * nkv * R * a.sp : 0, ls = a.weight ? B * nkv * R : 0;
+  const int64_t sc = a.weight ? B * nkv * R * a.sp : 0, ls = a.weight ? 2 * B * nkv * R : 0;
   at::Tensor ws = at::empty({po + ml + sc + ls + B + 1}, f32);
   a.part_o = ws.data_ptr<float>();
   a.part_ml = a.part_o + po;
   if (a.weight) {
     a.scores = a.part_ml + ml;
-    a.lse = a.scores + sc;
+    a.norm = a.scores + sc;
   }
   a.prefix = reinterpret_cast<int*>(a.part_ml + ml + sc + ls);
   const int rc = kv_attn_launch(a, dt, stream());

@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(32 * simt_warps<HDP>(), HDP == 512 ? 1 : 2) kv
       const long slot = 2L * blockIdx.x + (first ? 1 : 0);
       const float inv = l == 0.f ? 0.f : 1.f / l;
       if (lane < nr) {
-        if (all && a.lse) a.lse[bh * R + r0 + lane] = lse2(m, l);
+        if (all && a.norm) reinterpret_cast<float2*>(a.norm)[bh * R + r0 + lane] = row_norm(m, l);
         if (!all) *reinterpret_cast<float2*>(a.part_ml + (slot * a.rows + lane) * 2) = make_float2(m, l);
       }
 #pragma unroll
@@ -435,7 +435,7 @@ template <typename T, int WPR, int PER>
 __global__ void __launch_bounds__(JT) kv_join_k(KvAttnArgs a, int row_blocks) {
   constexpr int JW = JT * PER, UR = PER == 4 ? 4 : 1;
   constexpr int RPB = JT / 32 / WPR, COLS = 4;     // rows of a block, columns of a lane at a time
-  __shared__ float s_x[JT * COLS];
+  __shared__ __align__(8) float s_x[JT * COLS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, R = a.T * a.group;
   const bool out = blockIdx.x < (unsigned)row_blocks;
   const int wb = blockIdx.x - row_blocks, nch = (a.S + a.T + JW - 1) / JW;
@@ -517,26 +517,26 @@ __global__ void __launch_bounds__(JT) kv_join_k(KvAttnArgs a, int row_blocks) {
     for (int q = warp; q < min(JT, R - q0); q += JT / 32) {
       const int row = q0 + q, rb = row / a.rows;
       const Pieces p = pieces(rb);
-      float x;
+      float2 x;
       if (p.c0 == p.c1) {
-        x = a.lse[bh * R + row];
+        x = reinterpret_cast<const float2*>(a.norm)[bh * R + row];
       } else {
         float M, L;
         row_sum(a, p, row - rb * a.rows, M, L);
-        x = lse2(M, L);
+        x = row_norm(M, L);
       }
-      if (lane == 0) s_x[q] = x;
+      if (lane == 0) *reinterpret_cast<float2*>(s_x + 2 * q) = x;
     }
     __syncthreads();
     for (int q = 0; q < min(JT, R - q0); q += UR) {
-      float e[UR];
+      float2 e[UR];
 #pragma unroll
-      for (int k = 0; k < UR; ++k) e[k] = q + k < JT && q0 + q + k < R ? s_x[q + k] : CUDART_INF_F;
+      for (int k = 0; k < UR; ++k) e[k] = q + k < JT && q0 + q + k < R ? *reinterpret_cast<const float2*>(s_x + 2 * (q + k)) : make_float2(0.f, 0.f);
       if (q0 + q > 0) load(q0 + q);
 #pragma unroll
       for (int k = 0; k < UR; ++k)
 #pragma unroll
-        for (int i = 0; i < PER; ++i) add[i] += q0 + q + k < R ? ex2(s[k][i] - e[k]) : 0.f;
+        for (int i = 0; i < PER; ++i) add[i] = fmaf(ex2(s[k][i] - e[k].x), e[k].y, add[i]);
     }
   }
 #pragma unroll

@@ -53,12 +53,13 @@ template <> S0_DEV uint32_t rest2<__half>(float lo, float hi, uint32_t packed) {
   const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&packed));
   return pack2<__half>(lo - v.x, hi - v.y);
 }
-// The reference that the exponentials of a row refer to lies `up` below a maximum of its scores (base 2), and moves when a
-// score passes it by `far`.  Probabilities are then at most 2^far.  fp16 keeps nothing below 2^-25, which the many small
-// ones of a long context are beside one large one: with the reference 2^11 down that is 2^-36 of the largest.
+// Probabilities of the tensor-core kernels: 2^((s - m) scale + up), s the products as they come.  m is a score of the row (the
+// difference is exact for the scores next to it, however large they are) and moves when one passes it by `lazy` in base 2.
+// fp16 keeps nothing below 2^-25, which the many small ones of a long context are beside one large one: 2^11 up that
+// is 2^-36 of the largest.
 template <typename T> struct Ref;
-template <> struct Ref<__nv_bfloat16> { static constexpr float up = 0.f, far = 8.f; };
-template <> struct Ref<__half> { static constexpr float up = 11.f, far = 15.f; };
+template <> struct Ref<__nv_bfloat16> { static constexpr float up = 0.f, lazy = 8.f, down = 1.f; };
+template <> struct Ref<__half> { static constexpr float up = 11.f, lazy = 4.f, down = 1.f / 2048; };  // down = 2^-up
 // exponent bits all ones: infinity or NaN
 template <typename T> struct Inf;
 template <> struct Inf<__nv_bfloat16> { static constexpr uint32_t mask = 0x7f80u; };
@@ -248,8 +249,9 @@ int launch_after(void (*k)(P...), unsigned blocks, int threads, cudaStream_t st,
   return (int)cudaLaunchKernelEx(&cfg, k, P(args)...);
 }
 
-// base-2 log-sum-exp of a row; +inf where it saw nothing, so that exp2(s - lse) is 0 there
-S0_DEV float lse2(float m, float l) { return l == 0.f ? CUDART_INF_F : m + log2f(l); }
+// What a row's weights need: p = 2^(s - x) y, (x, y) = (maximum, 1 / sum) and (0, 0) where it saw nothing.  Apart, since a
+// sum's logarithm would lose its bits in that of a large maximum.
+S0_DEV float2 row_norm(float m, float l) { return make_float2(m == -CUDART_INF_F ? 0.f : m, l == 0.f ? 0.f : 1.f / l); }
 
 }  // namespace kv
 }  // namespace s0

@@ -42,7 +42,7 @@ constexpr int ST = 256, LT = 64, NT = ST + 32 + LT + 32;   // softmax threads, l
 constexpr int TM_O = 2 * N, TM_COLS = 256;            // tensor memory: S^T buffers at 0 and N, O^T
 constexpr unsigned long long DRAIN_NS = 2000000000ull;  // the bound of the wait for the last products, whatever the others' is
 __device__ int gave_up;                               // 1 once a wait has run out on this device
-constexpr float UNSET = -1e30f;                       // the reference of a row that has seen nothing
+constexpr float UNSET = -3.402823466e38f;                       // the reference of a row that has seen nothing
 
 template <int HD> struct Ring {
   static constexpr int SLOT = HD / 64 * PANEL, SLOTS = HD == 128 ? 5 : 8;
@@ -375,10 +375,9 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
 #pragma unroll
         for (int c = 0; c < W; c += 4) {
           const float4 m = *reinterpret_cast<const float4*>(m_ + c);
-          over = fmaxf(over, fmaxf(fmaxf(fmaf(s[c], a.scale_log2, -m.x), fmaf(s[c + 1], a.scale_log2, -m.y)),
-                                   fmaxf(fmaf(s[c + 2], a.scale_log2, -m.z), fmaf(s[c + 3], a.scale_log2, -m.w))));
+          over = fmaxf(over, fmaxf(fmaxf(s[c] - m.x, s[c + 1] - m.y), fmaxf(s[c + 2] - m.z, s[c + 3] - m.w)));
         }
-        const bool move = any_of(over > Ref<T>::far);
+        const bool move = any_of(over * a.scale_log2 > Ref<T>::lazy);
         if (i > 0) dead |= !wait(&bars.pdone, (i - 1) & 1, abort, a.wait_ns);  // P and O^T of the tile before are done with
         if (move) {
           float x[W];
@@ -387,9 +386,9 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
           s_l[quarter * N + half * W + lane] = transpose_reduce<true>(x, lane);
           softmax_sync();
           if (tid < N) {
-            const float x = fmaxf(fmaxf(s_l[tid], s_l[N + tid]), fmaxf(s_l[2 * N + tid], s_l[3 * N + tid])) * a.scale_log2 - Ref<T>::up;
+            const float x = fmaxf(fmaxf(s_l[tid], s_l[N + tid]), fmaxf(s_l[2 * N + tid], s_l[3 * N + tid]));
             const float was = s_m[tid], now = fmaxf(was, x);
-            s_al[tid] = ex2(was - now);
+            s_al[tid] = ex2((was - now) * a.scale_log2);
             s_m[tid] = now;
           }
           softmax_sync();
@@ -414,7 +413,7 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
           float p[8];
 #pragma unroll
           for (int x = 0; x < 8; ++x) {
-            p[x] = ex2(fmaf(s[c + x], a.scale_log2, -m[x]));
+            p[x] = ex2(fmaf(s[c + x] - m[x], a.scale_log2, Ref<T>::up));
             l[c + x] += p[x];
           }
           *reinterpret_cast<uint4*>(sP + kt * 128 + (((half * (W / 8) + (c >> 3)) ^ (kt & 7)) << 4)) =
@@ -445,11 +444,11 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
       if (any_of(dead)) break;
       if (tid < N) {
         const float x = (s_l[tid] + s_l[N + tid]) + (s_l[2 * N + tid] + s_l[3 * N + tid]);
-        const float m = s_m[tid] == UNSET ? -CUDART_INF_F : s_m[tid];
-        s_al[tid] = !all ? 1.f : x == 0.f ? 0.f : 1.f / x;
+        const float m = s_m[tid] == UNSET ? -CUDART_INF_F : s_m[tid] * a.scale_log2;
+        s_al[tid] = !all ? Ref<T>::down : x == 0.f ? 0.f : 1.f / x;
         if (r0 + tid < R) {
-          if (!all) *reinterpret_cast<float2*>(a.part_ml + (slot * a.rows + tid) * 2) = make_float2(m, x);
-          else if (a.lse) a.lse[bh * R + r0 + tid] = lse2(m, x);
+          if (!all) *reinterpret_cast<float2*>(a.part_ml + (slot * a.rows + tid) * 2) = make_float2(m, x * Ref<T>::down);
+          else if (a.norm) reinterpret_cast<float2*>(a.norm)[bh * R + r0 + tid] = row_norm(m, x * Ref<T>::down);
         }
       }
       softmax_sync();
@@ -490,7 +489,7 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
         float* p = a.part_o + (slot * a.rows + half * W) * a.hd + d;
 #pragma unroll
         for (int c = 0; c < W; ++c) {
-          if (q0 + c < R) *p = o[c];
+          if (q0 + c < R) *p = o[c] * Ref<T>::down;
           p += a.hd;
         }
       }
@@ -514,8 +513,8 @@ __global__ void __launch_bounds__(NT, 1) kv_attn_t5_k(KvAttnArgs a, int ctas) {
           const int row = r0 + e / a.hd, tok = div_group(a, row);
           ((T*)a.o)[(((long)cur.b * a.T + tok) * a.nkv * a.group + h * a.group + row - tok * a.group) * a.hd + e % a.hd] = Elem<T>::of(CUDART_NAN_F);
         }
-        if (a.lse)
-          for (int r = tid; r < nr; r += NT) a.lse[((long)cur.b * a.nkv + h) * R + r0 + r] = CUDART_NAN_F;
+        if (a.norm)
+          for (int r = tid; r < nr; r += NT) reinterpret_cast<float2*>(a.norm)[((long)cur.b * a.nkv + h) * R + r0 + r] = make_float2(0.f, CUDART_NAN_F);
       } else {
         for (int r = tid; r < nr; r += NT)
           *reinterpret_cast<float2*>(a.part_ml + ((2L * blockIdx.x + (cur.t == 0 ? 1 : 0)) * a.rows + r) * 2) = make_float2(0.f, CUDART_NAN_F);

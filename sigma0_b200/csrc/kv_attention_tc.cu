@@ -259,19 +259,19 @@ __global__ void __launch_bounds__(32 * WARPS, 2) kv_attn_tc_k(KvAttnArgs a, int 
             float x = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
 #pragma unroll
             for (int q = 1; q < KG; ++q) x = fmaxf(x, fmaxf(s[q][nt][e], s[q][nt][2 + e]));
-            mx[nt][e] = x * a.scale_log2;
-            far |= mx[nt][e] > m[nt][e] + Ref<T>::far;
+            mx[nt][e] = x;
+            far |= (x - m[nt][e]) * a.scale_log2 > Ref<T>::lazy;
           }
         if (__any_sync(0xffffffffu, far)) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float x = fmaxf(mx[nt][e] - Ref<T>::up, m[nt][e]);
+              float x = fmaxf(mx[nt][e], m[nt][e]);
               x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
               x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
               x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-              const float al = x == -CUDART_INF_F ? 1.f : ex2(m[nt][e] - x);
+              const float al = x == -CUDART_INF_F ? 1.f : ex2((m[nt][e] - x) * a.scale_log2);
               m[nt][e] = x;
               l[nt][e] *= al;
 #pragma unroll
@@ -289,8 +289,8 @@ __global__ void __launch_bounds__(32 * WARPS, 2) kv_attn_tc_k(KvAttnArgs a, int 
           for (int q = 0; q < KG; ++q)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              const float p0 = ex2(fmaf(s[q][nt][2 * x], a.scale_log2, -b0));
-              const float p1 = ex2(fmaf(s[q][nt][2 * x + 1], a.scale_log2, -b1));
+              const float p0 = ex2(fmaf(s[q][nt][2 * x] - b0, a.scale_log2, Ref<T>::up));
+              const float p1 = ex2(fmaf(s[q][nt][2 * x + 1] - b1, a.scale_log2, Ref<T>::up));
               l[nt][0] += p0;
               l[nt][1] += p1;
               const uint32_t p = pack2<T>(p0, p1);
@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(32 * WARPS, 2) kv_attn_tc_k(KvAttnArgs a, int 
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float m2 = ml[nt * 16 + 2 * e], x = fmaxf(m[nt][e], m2);
-          const float e0 = x == -CUDART_INF_F ? 1.f : ex2(m[nt][e] - x), e1 = x == -CUDART_INF_F ? 0.f : ex2(m2 - x);
+          const float e0 = x == -CUDART_INF_F ? 1.f : ex2((m[nt][e] - x) * a.scale_log2), e1 = x == -CUDART_INF_F ? 0.f : ex2((m2 - x) * a.scale_log2);
           m[nt][e] = x;
           l[nt][e] = l[nt][e] * e0 + ml[nt * 16 + 2 * e + 1] * e1;
 #pragma unroll
@@ -399,14 +399,14 @@ __global__ void __launch_bounds__(32 * WARPS, 2) kv_attn_tc_k(KvAttnArgs a, int 
 #pragma unroll
             for (int i = 0; i < HD / 8; ++i)
               if (i * 8 < a.hd) p[i * 8] = Elem<T>::of(o[i >> 1][nt][(i & 1) * 2 + e] * inv);
-            if (a.lse && g == 0) a.lse[bh * R + row] = lse2(m[nt][e], l[nt][e]);
+            if (a.norm && g == 0) reinterpret_cast<float2*>(a.norm)[bh * R + row] = row_norm(m[nt][e] * a.scale_log2, l[nt][e] * Ref<T>::down);
           } else {
             const long at = slot * a.rows + row - r0;
             float* p = a.part_o + at * a.hd + g;
 #pragma unroll
             for (int i = 0; i < HD / 8; ++i)
-              if (i * 8 < a.hd) p[i * 8] = o[i >> 1][nt][(i & 1) * 2 + e];
-            if (g == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m[nt][e], l[nt][e]);
+              if (i * 8 < a.hd) p[i * 8] = o[i >> 1][nt][(i & 1) * 2 + e] * Ref<T>::down;
+            if (g == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m[nt][e] * a.scale_log2, l[nt][e] * Ref<T>::down);
           }
         }
     }

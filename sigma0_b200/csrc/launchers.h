@@ -375,8 +375,8 @@ struct KvAttnArgs {
   // unit besides its tiles, its least cost, one CTA per unit (no split), kernel (0 fp32, 1 mma.sync, 2 tcgen05), 16-byte loads of floats
   int rows, nrb, tile, ctas, min_per, extra, least, whole, tc, vec;
   // scratch: 2 * ctas pieces of [rows, hd] and [rows, 2]; with weights [B, nkv, T * group, sp] scores
-  // and [B, nkv, T * group] log-sum-exps
-  float *part_o, *part_ml, *scores, *lse;
+  // and [B, nkv, T * group, 2] maxima and inverse sums of the rows that no join sees
+  float *part_o, *part_ml, *scores, *norm;
   int* prefix;                        // [B + 1] tiles of one (head, row block) before every sequence
   long sp;
   float inv_group;                    // 1 / group

@@ -64,3 +64,24 @@ def test_one_dominant_token_beside_a_long_tail(T, drop, dtype):
     if dtype == FH:
         bound += 2.0 ** -25 + n * 2.0 ** -36 * 6  # |v| below 6
     assert ((o - o64).norm(dim=-1) <= bound.norm(dim=-1)).all(), ((o - o64).norm() / bound.norm()).item()
+
+
+@pytest.mark.parametrize("dtype,e", [(BF, 4), (BF, 20), (BF, 52), (FH, 4), (FH, 15), (torch.float32, 20), (torch.float32, 52)])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("T,n", [(1, 400), (1, 30000), (12, 3000), (40, 400), (40, 30000)])
+def test_scores_of_any_size(T, n, sign, dtype, e):
+    """Half of the keys have the score sign 2^(2 e + 3) exactly, the others one that is lower by 2^-7 of it or more: the output
+    is the mean of the first half's values and their weights are equal, whatever the size of the scores."""
+    from sigma0_b200.ops.kv_cache import cache_attention
+    nkv, hd = 2, 64
+    S = n + T
+    q = torch.full((1, T, nkv, hd), 2.0 ** e, device="cuda", dtype=dtype)
+    kc = torch.full((1, nkv, S, hd), sign * 2.0 ** e, device="cuda", dtype=dtype)
+    kc[:, :, 1::2] = sign * 2.0 ** e * (1 - sign * 2.0 ** -7)
+    kn = torch.full_like(q, sign * 2.0 ** e * (1 - sign * 2.0 ** -7))
+    vc, vn = _rand(T, kc.shape, q.shape, dtype=dtype)
+    ls = torch.tensor([n], dtype=torch.int32, device="cuda")
+    o64, w64 = K.attention(q, kn, vn, kc, vc, [n], None, 0.125)
+    w = torch.zeros(1, nkv, S, device="cuda")
+    o = cache_attention(q, kn, vn, kc, vc, ls, scale=0.125, weight=w)
+    assert K.rel(o, o64) < K.tolerance(dtype) and K.rel(w, w64) < K.WEIGHT_TOL
