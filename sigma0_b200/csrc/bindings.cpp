@@ -4,6 +4,7 @@
 // torch-free kernels and raw-pointer launchers (launchers.h).
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <algorithm>
 #include <atomic>
@@ -783,6 +784,21 @@ static void kv_slots(const at::Tensor& t, const char* name, at::ScalarType dt, c
   TORCH_CHECK(t.sizes() == kc.sizes().slice(0, kc.dim() - 1) && (t.stride(-1) == 1 || t.size(-1) <= 1), name,
               " must have the cache's shape without the head dimension, slots contiguous");
 }
+// a tensor that is written must not hold one element at several indexes: blocks would race for it
+static void kv_apart(const at::Tensor& t, const char* name) {
+  int64_t span = 1;
+  bool zero = false;
+  for (int64_t d = 0; d < t.dim(); ++d) {
+    span += (t.size(d) - 1) * t.stride(d);
+    zero |= t.size(d) > 1 && t.stride(d) == 0;
+  }
+  TORCH_CHECK(t.numel() == 0 || (!zero && span >= t.numel()), name, " is written: it must not be expanded");
+}
+// an output: none of the elements that are read for others, unless it is that input
+static void kv_output(const at::Tensor& out, const at::Tensor& in, const char* name) {
+  const auto o = at::get_overlap_status(out, in);
+  TORCH_CHECK(o != at::MemOverlapStatus::Partial, name, " output overlaps its input: the whole of it or nothing");
+}
 // a cache [B, nkv, S, hd] is one of a single layer
 static int64_t kv_layers(const at::Tensor& t, int64_t rank) { return t.dim() == rank ? t.size(0) : 1; }
 static int64_t kv_layer_stride(const at::Tensor& t, int64_t rank) { return t.dim() == rank ? t.stride(0) : 0; }
@@ -846,11 +862,13 @@ at::Tensor kv_attn(at::Tensor q, at::Tensor kn, at::Tensor vn, at::Tensor kc, at
   }
   if (weight && weight->defined()) {
     kv_slots(*weight, "weight", at::kFloat, kc);
+    kv_apart(*weight, "weight");
     a.weight = weight->data_ptr<float>();
     a.wt_b = weight->stride(0); a.wt_h = weight->stride(1);
   }
   if (positions && positions->defined()) {
     kv_slots(*positions, "positions", at::kInt, kc);
+    kv_apart(*positions, "positions");
     TORCH_CHECK(seen && seen->defined(), "positions need seen");
     kv_ints(*seen, "seen", B, dev);
     a.positions = positions->data_ptr<int>();
@@ -899,6 +917,8 @@ std::vector<at::Tensor> kv_evict(at::Tensor kc, at::Tensor vc, at::Tensor weight
   kv_caches(kc, vc, true);
   const auto dev = kc.device();
   const int64_t N = kv_layers(kc, 5), B = kc.size(-4), nkv = kc.size(-3), S = kc.size(-2), hd = kc.size(-1);
+  kv_apart(kc, "k_cache");
+  kv_apart(vc, "v_cache");
   kv_slots(weight, "weight", at::kFloat, kc);
   kv_slots(positions, "positions", at::kInt, kc);
   kv_ints(lengths, "lengths", B, dev);
@@ -913,6 +933,12 @@ std::vector<at::Tensor> kv_evict(at::Tensor kc, at::Tensor vc, at::Tensor weight
   kv_slots(wo, "weight output", at::kFloat, kc);
   kv_slots(po, "positions output", at::kInt, kc);
   kv_ints(lo, "lengths output", B, dev);
+  kv_apart(wo, "weight output");
+  kv_apart(po, "positions output");
+  kv_output(wo, weight, "weight");
+  kv_output(po, positions, "positions");
+  kv_output(lo, lengths, "lengths");
+  TORCH_CHECK(B == 0 || at::get_overlap_status(lo, seen) == at::MemOverlapStatus::No, "the lengths output must not be seen");
   TORCH_CHECK((wo.data_ptr() != weight.data_ptr() || wo.strides() == weight.strides()) &&
                   (po.data_ptr() != positions.data_ptr() || po.strides() == positions.strides()),
               "an output that is its input must be the whole of it");
@@ -946,6 +972,8 @@ std::vector<at::Tensor> kv_commit(at::Tensor parents, at::Tensor tokens, at::Ten
   kv_caches(kc, vc, true);
   const auto dev = kc.device();
   const int64_t N = kv_layers(kc, 5), B = kc.size(-4), nkv = kc.size(-3), S = kc.size(-2), hd = kc.size(-1);
+  kv_apart(kc, "k_cache");
+  kv_apart(vc, "v_cache");
   req(tokens, at::kLong, "tokens");
   req(targets, at::kLong, "targets");
   TORCH_CHECK(tokens.dim() == 2 && tokens.size(0) == B && targets.sizes() == tokens.sizes() && tokens.device() == dev &&
@@ -959,11 +987,13 @@ std::vector<at::Tensor> kv_commit(at::Tensor parents, at::Tensor tokens, at::Ten
   KvCommitArgs a{};
   if (weight && weight->defined()) {
     kv_slots(*weight, "weight", at::kFloat, kc);
+    kv_apart(*weight, "weight");
     a.weight = weight->data_ptr<float>();
     a.w_n = kv_layer_stride(*weight, 4); a.w_b = weight->stride(-3); a.w_h = weight->stride(-2);
   }
   if (positions && positions->defined()) {
     kv_slots(*positions, "positions", at::kInt, kc);
+    kv_apart(*positions, "positions");
     TORCH_CHECK(seen && seen->defined(), "positions need seen");
     kv_ints(*seen, "seen", B, dev);
     a.positions = positions->data_ptr<int>();

@@ -61,7 +61,7 @@ def cache_attention(q, k_new, v_new, k_cache, v_cache, lengths, mask=None, scale
 
     ``weight`` [B, kv_heads, slots] gets the probabilities of all T rows and of the group's query heads
     added (through a scratch of 4 bytes per row and slot), ``positions`` the value ``seen[b] + i`` for new
-    token i; both in place.  ``scale`` must be positive; k_new and v_new must not overlap the caches."""
+    token i; both in place, so neither may be expanded.  ``scale`` must be positive; k_new and v_new must not overlap the caches."""
     _inference_only(q, k_new, v_new, k_cache, v_cache)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if k_cache.is_cuda:
@@ -77,7 +77,7 @@ def cache_evict(k_cache, v_cache, weight, positions, lengths, seen, keep, recent
     ``weight`` (the lower slot among equals; NaN counts as the most).  Rows of survivors behind the new
     end move into free slots before it, in place.  A sequence of at most ``keep`` tokens stays as it is.
     Slots from the new length on get weight 0 and position -1.  ``out``: three tensors for the results,
-    which may be the inputs themselves."""
+    which may be the inputs themselves but not a part of them."""
     if k_cache.is_cuda:
         ow, op, ol = out if out is not None else (None, None, None)
         return tuple(ext().kv_evict(k_cache, v_cache, weight, positions, lengths, seen, keep, recent, sinks, ow, op, ol))
@@ -87,6 +87,7 @@ def cache_evict(k_cache, v_cache, weight, positions, lengths, seen, keep, recent
     res = (w, p, n) if layers else (w[0], p[0], n)
     if out is None:
         return res
+    _apart(*zip(("weight output", "positions output", "lengths output"), out))
     for o, r in zip(out, res):
         o.copy_(r)
     return tuple(out)
@@ -202,6 +203,14 @@ def wait_limit(seconds: float = 2.0) -> None:
 
 
 # ---- torch expressions (CPU tensors) ------------------------------------------------------------
+def _apart(*named):
+    for name, t in named:
+        if t is not None and t.numel():
+            span = 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+            if span < t.numel() or any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+                raise ValueError(f"{name} is written: it must not be expanded")
+
+
 def _attention_torch(q, k_new, v_new, kc, vc, lengths, mask, scale, weight, positions, seen):
     B, T, nh, hd = q.shape
     nkv, S = kc.shape[1], kc.shape[2]
@@ -209,6 +218,7 @@ def _attention_torch(q, k_new, v_new, kc, vc, lengths, mask, scale, weight, posi
         raise ValueError("q, k_new and v_new must match the caches' batch, kv heads and head dim")
     if positions is not None and seen is None:
         raise ValueError("positions need seen")
+    _apart(("weight", weight), ("positions", positions))
     new = torch.ones(T, T, dtype=torch.bool).tril() if mask is None else mask
     new = new.expand(B, T, T)
     o = torch.zeros(B, T, nh, hd, dtype=q.dtype)
@@ -238,6 +248,7 @@ def _attention_torch(q, k_new, v_new, kc, vc, lengths, mask, scale, weight, posi
 def _evict_torch(kc, vc, w, pos, lengths, seen, keep, recent, sinks):
     if keep < 1 or recent < 0 or sinks < 0 or recent + sinks > keep:
         raise ValueError("keep >= 1 and recent + sinks <= keep")
+    _apart(("k_cache", kc), ("v_cache", vc))
     S = w.shape[-1]
     slot = torch.arange(S)
     ls = lengths.long().clamp(0, S)[:, None, None]
@@ -262,6 +273,7 @@ def _evict_torch(kc, vc, w, pos, lengths, seen, keep, recent, sinks):
 def _commit_torch(parents, tokens, targets, kc, vc, lengths, weight, positions, seen):
     if positions is not None and seen is None:
         raise ValueError("positions need seen")
+    _apart(("k_cache", kc), ("v_cache", vc), ("weight", weight), ("positions", positions))
     B, T = tokens.shape
     S = kc.shape[3]
     par = parents.expand(B, T).tolist()
