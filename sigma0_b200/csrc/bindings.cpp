@@ -853,12 +853,13 @@ at::Tensor kv_attn(at::Tensor q, at::Tensor kn, at::Tensor vn, at::Tensor kc, at
   kv_ints(lengths, "lengths", B, dev);
   KvAttnArgs a{};
   if (mask && mask->defined()) {
-    TORCH_CHECK(mask->device() == dev && mask->scalar_type() == at::kBool && mask->is_contiguous() &&
+    TORCH_CHECK(mask->device() == dev && mask->scalar_type() == at::kBool &&
+                    (mask->dim() == 2 || (mask->dim() == 3 && (mask->size(0) == B || mask->size(0) == 1))) &&
                     mask->size(-1) == T && mask->size(-2) == T &&
-                    (mask->dim() == 2 || (mask->dim() == 3 && (mask->size(0) == B || mask->size(0) == 1))),
-                "mask: contiguous bool [T, T] or [B, T, T]");
+                    (T <= 1 || (mask->stride(-1) == 1 && mask->stride(-2) == T)),
+                "mask: bool [T, T] or [B, T, T], a sequence's part contiguous");
     a.mask = reinterpret_cast<const unsigned char*>(mask->data_ptr<bool>());
-    a.mask_b = mask->dim() == 3 && mask->size(0) == B && B > 1 ? T * T : 0;
+    a.mask_b = mask->dim() == 3 && mask->size(0) > 1 ? mask->stride(0) : 0;
   }
   if (weight && weight->defined()) {
     kv_slots(*weight, "weight", at::kFloat, kc);

@@ -56,7 +56,7 @@ def cache_attention(q, k_new, v_new, k_cache, v_cache, lengths, mask=None, scale
     q [B, T, heads, hd], k_new / v_new [B, T, kv_heads, hd], caches [B, kv_heads, slots, hd], all of one
     dtype (float32, float16, bfloat16; hd <= 512, T <= 1024) and ``heads`` a multiple of ``kv_heads``.
     Every new token sees the ``lengths[b]`` cached ones and those new ones that its row of ``mask``
-    (bool [T, T] or [B, T, T]; None: causal) names; a row that sees nothing gives zeros, and a NaN or an
+    (bool [T, T] or [B, T, T], which may be expanded over the sequences; None: causal) names; a row that sees nothing gives zeros, and a NaN or an
     infinity in a token shows in no row that does not see it.  The new rows are stored in slots ``lengths[b] ...``; rows past the last slot are attended to but not stored.
 
     ``weight`` [B, kv_heads, slots] gets the probabilities of all T rows and of the group's query heads
@@ -211,13 +211,47 @@ def _apart(*named):
                 raise ValueError(f"{name} is written: it must not be expanded")
 
 
+def _ints(*named, shape=None):
+    for name, t in named:
+        if t.dtype != torch.int32 or not t.is_contiguous() or t.shape != shape:
+            raise ValueError(f"{name}: contiguous int32 {list(shape)}")
+
+
+def _caches(kc, vc, layers, weight=None, positions=None):
+    """What the CUDA entry points ask of the caches and of the tensors of their slots."""
+    if kc.dim() not in ((4, 5) if layers else (4,)) or kc.shape != vc.shape or kc.dtype != vc.dtype:
+        raise ValueError("the caches must have one shape and one dtype")
+    if kc.dtype not in (torch.float32, torch.float16, torch.bfloat16) or not kc.shape[-1]:
+        raise ValueError("caches of float32, float16 or bfloat16")
+    if kc.stride(-1) != 1 or vc.stride(-1) != 1:
+        raise ValueError("the caches' head dimension must be contiguous")
+    for name, t, dt in (("weight", weight, torch.float32), ("positions", positions, torch.int32)):
+        if t is not None and (t.dtype != dt or t.shape != kc.shape[:-1] or (t.shape[-1] > 1 and t.stride(-1) != 1)):
+            raise ValueError(f"{name}: {dt} of the cache's shape without the head dimension, slots contiguous")
+
+
 def _attention_torch(q, k_new, v_new, kc, vc, lengths, mask, scale, weight, positions, seen):
+    _caches(kc, vc, False, weight, positions)
+    if q.dim() != 4 or q.shape[0] != kc.shape[0] or q.shape[3] != kc.shape[3]:
+        raise ValueError("q, k_new and v_new must match the caches' batch, kv heads and head dim")
     B, T, nh, hd = q.shape
     nkv, S = kc.shape[1], kc.shape[2]
+    if any(t.dtype != kc.dtype or t.stride(-1) != 1 for t in (q, k_new, v_new)):
+        raise ValueError("q, k_new and v_new: the caches' dtype, contiguous head dimension")
+    if hd > 512 or T > 1024 or B > 8192 or not nkv or nh > 1024 * nkv:
+        raise ValueError("head dim up to 512, 1024 new tokens, 1024 heads over one kv head, 8192 sequences")
+    if not 0 < scale < 1e30:
+        raise ValueError("scale must be positive")
+    _ints(("lengths", lengths), shape=(B,))
+    if mask is not None and (mask.dtype != torch.bool or mask.shape not in ((T, T), (B, T, T), (1, T, T))
+                             or (T > 1 and mask.stride()[-2:] != (T, 1))):
+        raise ValueError("mask: bool [T, T] or [B, T, T], a sequence's part contiguous")
     if nh % nkv or k_new.shape != (B, T, nkv, hd) or v_new.shape != k_new.shape or kc.shape != vc.shape:
         raise ValueError("q, k_new and v_new must match the caches' batch, kv heads and head dim")
     if positions is not None and seen is None:
         raise ValueError("positions need seen")
+    if positions is not None:
+        _ints(("seen", seen), shape=(B,))
     _apart(("weight", weight), ("positions", positions))
     new = torch.ones(T, T, dtype=torch.bool).tril() if mask is None else mask
     new = new.expand(B, T, T)
@@ -248,6 +282,8 @@ def _attention_torch(q, k_new, v_new, kc, vc, lengths, mask, scale, weight, posi
 def _evict_torch(kc, vc, w, pos, lengths, seen, keep, recent, sinks):
     if keep < 1 or recent < 0 or sinks < 0 or recent + sinks > keep:
         raise ValueError("keep >= 1 and recent + sinks <= keep")
+    _caches(kc, vc, True, w, pos)
+    _ints(("lengths", lengths), ("seen", seen), shape=(kc.shape[1],))
     _apart(("k_cache", kc), ("v_cache", vc))
     S = w.shape[-1]
     slot = torch.arange(S)
@@ -274,8 +310,17 @@ def _commit_torch(parents, tokens, targets, kc, vc, lengths, weight, positions, 
     if positions is not None and seen is None:
         raise ValueError("positions need seen")
     _apart(("k_cache", kc), ("v_cache", vc), ("weight", weight), ("positions", positions))
+    _caches(kc, vc, True, weight, positions)
+    if tokens.dim() != 2 or tokens.shape[0] != kc.shape[1] or targets.shape != tokens.shape:
+        raise ValueError("tokens and targets: int64 [B, T]")
     B, T = tokens.shape
     S = kc.shape[3]
+    if any(t.dtype != torch.int64 or not t.is_contiguous() for t in (tokens, targets)) or not 1 <= T <= 1024 or not kc.shape[0]:
+        raise ValueError("tokens and targets: contiguous int64 [B, T], 1 to 1024 nodes, at least one layer")
+    _ints(("parents", parents), shape=(T,) if parents.dim() == 1 else (B, T))
+    _ints(("lengths", lengths), shape=(B,))
+    if positions is not None:
+        _ints(("seen", seen), shape=(B,))
     par = parents.expand(B, T).tolist()
     path = torch.full((B, T), -1, dtype=torch.int32)
     count = torch.empty(B, dtype=torch.int32)
