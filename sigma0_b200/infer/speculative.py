@@ -1,11 +1,12 @@
 """Greedy generation of transformer stacks with drafted trees and a token budget.
 
 A step of :class:`TreeDecoder` takes the last token and a tree of drafts through the whole model at
-once, accepts the longest path that the model itself would have produced, and cuts the caches to
+once, accepts the path that the model itself would have produced, and cuts the caches to
 their budget (:mod:`sigma0_b200.ops.kv_cache`).  Without a budget the tokens are those of one-by-one
 greedy decoding; drafts only change how many of them a step yields.  Drafts come from the
 sequence itself: what followed the latest earlier occurrences of its last two tokens, which order
-flow with its repeated message skeletons offers often.
+flow with its repeated message skeletons offers often.  Several of them often begin alike; they share
+the nodes of what they have in common, so that the model's path is in the tree if one of them has it.
 
 ``python -m sigma0_b200.infer.speculative --help`` runs it on a random-init model.  The reference
 generates one token per model call (``src/base_model/inference/generate.py:870-1061``).
@@ -19,7 +20,7 @@ import time
 import torch
 
 from ..models.transformer import TransformerBlock
-from ..ops.kv_cache import KVCache, check, tree_depth, tree_mask
+from ..ops.kv_cache import KVCache, check, tree_depth
 
 
 class TreeDecoder:
@@ -133,6 +134,34 @@ def chain_tree(width, depth, device=None):
     return torch.tensor(par, dtype=torch.int32, device=device)
 
 
+def merge_tables(batch, width, depth, device=None):
+    """What :func:`merged_tree` needs beside the drafts, which a generation makes once."""
+    at = torch.arange(depth, device=device)
+    parents = chain_tree(width, depth, device).repeat(batch, 1)
+    mask = torch.zeros(batch, parents.shape[1], parents.shape[1], dtype=torch.bool, device=device)
+    mask[:, :, 0] = True
+    return at + 1, at <= at[:, None], torch.arange(width, device=device)[:, None], parents, mask
+
+
+def merged_tree(drafts, width, depth, tables=None):
+    """The ``width`` chains of ``drafts`` (B, width * depth) with equal beginnings merged, as
+    :func:`chain_tree` numbers their nodes -> (parents int32 (B, T), mask bool (B, T, T), drafts).
+
+    A node that repeats a lower chain's up to there is left out: its draft becomes -1, which no model says, and what
+    follows hangs below the lower chain's.  So no two children of a node carry the same token, and the walk of
+    :func:`~sigma0_b200.ops.kv_cache.tree_commit` misses no longer path."""
+    B = drafts.shape[0]
+    place, upto, chain, parents, mask = tables or merge_tables(B, width, depth, drafts.device)
+    d = drafts.reshape(B, width, depth)
+    first = (d[:, :, None] == d[:, None]).cumprod(-1).argmax(2)           # the lowest chain that agrees up to here
+    node = torch.add(place, first, alpha=depth)                           # the node that stands for (chain, depth)
+    parents, mask = parents.clone(), mask.clone()
+    parents[:, 1:].unflatten(1, (width, depth))[..., 1:] = node[..., :-1]
+    up = torch.where(upto, node[:, :, None], 0)                           # those of a chain down to here; the root
+    mask[:, 1:].scatter_(2, up.reshape(B, width * depth, depth), True)
+    return parents, mask, torch.where(first == chain, d, -1).reshape(B, -1)
+
+
 @torch.no_grad()
 def generate(decoder: TreeDecoder, prompt, n, book=None, width=2, depth=6, chunk=512):
     """Greedy tokens (B, n) after ``prompt`` (B, L) and the steps that they took.
@@ -149,13 +178,15 @@ def generate(decoder: TreeDecoder, prompt, n, book=None, width=2, depth=6, chunk
     history[:, :L] = prompt
     length = torch.full((B,), L, dtype=torch.long, device=dev)
     last = decoder.prefill(prompt, book, chunk)
-    parents = chain_tree(width, depth, dev)
-    mask = tree_mask(parents)
+    parents, mask = chain_tree(width, depth, dev), None                   # the root alone
+    tables = merge_tables(B, width, depth, dev)
     history[:, L] = last
     length += 1
     steps, at = 0, torch.arange(nodes, device=dev)
     while int((length - L).min()) < n:
-        drafts = lookup_drafts(history, length, width, depth) if depth else history.new_zeros(B, 0)
+        drafts = history.new_zeros(B, 0)
+        if nodes > 1:
+            parents, mask, drafts = merged_tree(lookup_drafts(history, length, width, depth), width, depth, tables)
         tokens = torch.cat([last[:, None], drafts], 1)
         logits = decoder.forward(tokens.clamp_min(0), book, mask)
         targets = logits.argmax(-1)

@@ -11,7 +11,7 @@ cache's shape without the head dimension, -1 in free slots) says which token a s
 * :func:`cache_attention` stores the keys and values of T new tokens in slots ``[len, len + T)``
   and attends from them; ``lengths`` stays as it is until the caller adds the tokens that it keeps.
 * :func:`cache_evict` cuts every layer and head to ``keep`` tokens by accumulated weight.
-* :func:`tree_commit` accepts the longest path of a drafted tree that agrees with the model.
+* :func:`tree_commit` accepts the path of a drafted tree that agrees with the model.
 * :class:`KVCache` holds the tensors of several layers and calls the three.
 
 CUDA tensors run the kernels of ``csrc/kv_attention.cu``, ``csrc/kv_attention_tc.cu`` and
@@ -94,11 +94,12 @@ def cache_evict(k_cache, v_cache, weight, positions, lengths, seen, keep, recent
 
 
 def tree_commit(parents, tokens, targets, k_cache, v_cache, lengths, weight=None, positions=None, seen=None):
-    """Accept the longest root path of a drafted tree that the model agrees with -> (path, count, token).
+    """Accept the root path of a drafted tree that the model agrees with -> (path, count, token).
 
     Node 0 of the T nodes is the last accepted token; node i hangs below node ``parents[i] < i`` (int32 [T]
     or [B, T]), drafts ``tokens[b, i]`` (int64) and the model continues it with ``targets[b, i]``.  From the
-    root the walk goes to the lowest child whose token is the model's, until there is none: ``path``
+    root the walk goes to the lowest child whose token is the model's, until there is none (where siblings carry
+    the same token, a longer path below the higher one is not seen: merge them): ``path``
     int32 [B, T] holds its nodes (-1 behind them), ``count`` int32 [B] how many, ``token`` int64 [B] the
     model's token after the last.  Nodes past the last slot have no rows and are not accepted; where not even
     the root has one, ``count`` is 0 and ``token`` the root's own.  The path's rows, which :func:`cache_attention` left in slots
