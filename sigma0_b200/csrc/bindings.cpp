@@ -943,7 +943,10 @@ std::vector<at::Tensor> kv_evict(at::Tensor kc, at::Tensor vc, at::Tensor weight
   TORCH_CHECK((wo.data_ptr() != weight.data_ptr() || wo.strides() == weight.strides()) &&
                   (po.data_ptr() != positions.data_ptr() || po.strides() == positions.strides()),
               "an output that is its input must be the whole of it");
-  if (N * B * nkv == 0) return {wo, po, lo};
+  if (N * B * nkv == 0) {                       // no layers or no heads: only the lengths change
+    lo.copy_(lengths.clamp(0, std::min(keep, S)));
+    return {wo, po, lo};
+  }
   const int64_t cap = std::min(keep, std::max<int64_t>(1, S));
   at::Tensor ws = at::empty({N * B * nkv * (2 * cap + 1)}, lengths.options());
   KvEvictArgs a{};
