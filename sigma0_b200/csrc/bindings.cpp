@@ -1013,6 +1013,7 @@ std::vector<at::Tensor> kv_commit(at::Tensor parents, at::Tensor tokens, at::Ten
   a.tokens = reinterpret_cast<const long*>(tokens.data_ptr<int64_t>());
   a.targets = reinterpret_cast<const long*>(targets.data_ptr<int64_t>());
   a.lengths = lengths.data_ptr<int>();
+  TORCH_CHECK(kc.data_ptr() != vc.data_ptr() || kc.strides() == vc.strides(), "k_cache and v_cache: one tensor or two");
   a.kc = kc.data_ptr(); a.vc = vc.data_ptr();
   a.path = path.data_ptr<int>(); a.count = count.data_ptr<int>();
   a.next = reinterpret_cast<long*>(next.data_ptr<int64_t>());

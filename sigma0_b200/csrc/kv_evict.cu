@@ -310,6 +310,7 @@ __global__ void __launch_bounds__(CT) commit_k(KvCommitArgs a) {
   // at a time (a destination never lies behind a later source)
   const int C = a.hd * a.esize / (int)sizeof(V);
   for (int i = tid; i < 2 * a.nkv * C; i += CT) {
+    if (i >= a.nkv * C && a.vc == a.kc) break;           // one tensor for keys and values moves once
     const int kv = i / (a.nkv * C), h = i / C % a.nkv;
     const long c = (long)(i % C) * sizeof(V);
     const long rs = (kv ? a.vc_s : a.kc_s) * a.esize;

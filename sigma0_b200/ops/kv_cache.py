@@ -104,7 +104,7 @@ def tree_commit(parents, tokens, targets, k_cache, v_cache, lengths, weight=None
     model's token after the last.  Nodes past the last slot have no rows and are not accepted; where not even
     the root has one, ``count`` is 0 and ``token`` the root's own.  The path's rows, which :func:`cache_attention` left in slots
     ``lengths[b] + node``, move up to ``lengths[b] + 0, 1, ...`` in all layers; ``weight`` follows and is 0
-    for the dropped ones, ``positions`` become ``seen[b] + 0, 1, ...`` and -1.  ``lengths`` and ``seen``
+    for the dropped ones, ``positions`` become ``seen[b] + 0, 1, ...`` and -1.  One tensor may be both caches.  ``lengths`` and ``seen``
     stay as they are: add ``count`` to them."""
     if k_cache.is_cuda:
         return tuple(ext().kv_commit(parents, tokens, targets, k_cache, v_cache, lengths, weight, positions, seen))
@@ -337,7 +337,7 @@ def _commit_torch(parents, tokens, targets, kc, vc, lengths, weight, positions, 
                 break
             walk.append(nxt)
         rows = torch.tensor([n + i for i in walk], dtype=torch.long)
-        for cache in (kc, vc):
+        for cache in (kc,) if kc.data_ptr() == vc.data_ptr() else (kc, vc):   # one tensor for both moves once
             cache[:, b, :, n:n + len(walk)] = cache[:, b].index_select(2, rows)
         if weight is not None:
             was = weight[:, b].index_select(2, rows)

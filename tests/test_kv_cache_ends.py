@@ -72,3 +72,19 @@ def test_a_cache_holds_the_accepted_tokens_and_no_others(dev, T, room):
         assert torch.equal(c.k[:, b, :, n0:n0 + n], rows) and torch.equal(c.v[:, b, :, n0:n0 + n], -rows)
         assert (c.positions[:, b, :, :n0 + n] == torch.arange(45, 50 + n, device=dev)).all()
         assert (c.positions[:, b, :, n0 + n:] == -1).all() and (c.weight[:, b, :, n0 + n:] == 0).all()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_one_tensor_for_keys_and_values(dev):
+    """Rows that follow one another move down a path whose nodes are others' destinations: each moves once."""
+    T, S = 300, 310
+    live = [i for i in range(T) if i % 3 != 2]                         # every third node is a draft that does not fit
+    par, tok = [0] * T, [5] * T
+    for k, i in enumerate(live):
+        par[i], tok[i] = live[k - 1] if k else -1, 0
+    par, tok = torch.tensor(par, dtype=torch.int32, device=dev), torch.tensor([tok], device=dev)
+    kc = torch.arange(float(S), device=dev)[:, None].expand(2, 1, 3, S, 8).contiguous()
+    path, count, _ = tree_commit(par, tok, torch.zeros_like(tok), kc, kc, torch.tensor([4], dtype=torch.int32, device=dev))
+    n = len(live)
+    assert path[0, :n].tolist() == live and int(count) == n
+    assert torch.equal(kc[..., 4:4 + n, 0], (torch.tensor(live, device=dev) + 4.0).expand(2, 1, 3, n))
