@@ -1693,6 +1693,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv_status", [](at::Tensor like) { return kv_status(like); },
         "status word of the tcgen05 cache attention (nonzero: a bounded wait ran out)");
   m.def("kv_wait_limit", &kv_wait_limit, py::arg("seconds"), "bound of the tcgen05 cache attention's waits");
+  m.def("kv_launches", [] { return (int64_t)kv_launches(); }, "kernels that the cache operators have launched so far");
   m.def("kv_evict", &kv_evict, py::arg("k_cache"), py::arg("v_cache"), py::arg("weight"), py::arg("positions"),
         py::arg("lengths"), py::arg("seen"), py::arg("keep"), py::arg("recent"), py::arg("sinks"),
         py::arg("weight_out"), py::arg("positions_out"), py::arg("lengths_out"),

@@ -550,7 +550,7 @@ int run_any(const KvAttnArgs& a, cudaStream_t st) {
   const cudaError_t e = cudaFuncSetAttribute(kv_attn_any_k<T, HDP, RB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
   if (e != cudaSuccess) return (int)e;
   kv_attn_any_k<T, HDP, RB><<<a.whole ? a.B * a.nkv * a.nrb : a.ctas, 32 * simt_warps<HDP>(), sm, st>>>(a, a.ctas);
-  return (int)cudaGetLastError();
+  return launched();
 }
 template <typename T, int HDP>
 int run_any_rows(const KvAttnArgs& a, cudaStream_t st) {
@@ -584,6 +584,8 @@ int join(const KvAttnArgs& a, cudaStream_t st) {
 
 }  // namespace kv
 }  // namespace s0
+
+long kv_launches() { return s0::kv::launches; }
 
 void kv_attn_plan(KvAttnArgs& a, int dtype, int sms) {
   if (kv_attn_tc_takes(a, dtype)) return kv_attn_tc_plan(a, sms);

@@ -17,12 +17,20 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math_constants.h>
+#include <atomic>
 
 #include "common.cuh"
 #include "launchers.h"
 
 namespace s0 {
 namespace kv {
+
+// kernels launched by these files, in all threads: a call takes one or two, by its sizes
+inline std::atomic<long> launches{0};
+inline int launched() {
+  ++launches;
+  return (int)cudaGetLastError();
+}
 
 template <typename T> struct Elem;
 template <> struct Elem<float> {
@@ -246,6 +254,7 @@ int launch_after(void (*k)(P...), unsigned blocks, int threads, cudaStream_t st,
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
+  ++launches;
   return (int)cudaLaunchKernelEx(&cfg, k, P(args)...);
 }
 

@@ -532,7 +532,7 @@ int run(const KvAttnArgs& a, cudaStream_t st) {
   const cudaError_t e = cudaFuncSetAttribute(kv_attn_t5_k<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
   if (e != cudaSuccess) return (int)e;
   kv_attn_t5_k<T, HD><<<a.whole ? a.B * a.nkv * a.nrb : a.ctas, NT, sm, st>>>(a, a.ctas);
-  return (int)cudaGetLastError();
+  return launched();
 }
 
 }  // namespace t5

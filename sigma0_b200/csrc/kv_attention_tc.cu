@@ -422,7 +422,7 @@ int run_tc(const KvAttnArgs& a, cudaStream_t st) {
   const cudaError_t e = cudaFuncSetAttribute(kv_attn_tc_k<T, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
   if (e != cudaSuccess) return (int)e;
   kv_attn_tc_k<T, HD, NT><<<a.whole ? a.B * a.nkv * a.nrb : a.ctas, 32 * WARPS, sm, st>>>(a, a.ctas);
-  return (int)cudaGetLastError();
+  return launched();
 }
 template <typename T, int HD>
 int launch_tc(const KvAttnArgs& a, cudaStream_t st) {

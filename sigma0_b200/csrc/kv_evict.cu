@@ -364,7 +364,7 @@ static int select_units(const KvEvictArgs& a, unsigned units, int moves_here, cu
   const cudaError_t e = cudaFuncSetAttribute(s0::kv::evict_k<NT, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
   if (e != cudaSuccess) return (int)e;
   s0::kv::evict_k<NT, KEYS><<<units, NT, sm, st>>>(a, moves_here);
-  return (int)cudaGetLastError();
+  return s0::kv::launched();
 }
 
 int kv_evict_launch(KvEvictArgs a, cudaStream_t st) {
@@ -395,5 +395,5 @@ int kv_commit_launch(const KvCommitArgs& a, cudaStream_t st) {
   else if (v == 8) commit_k<uint2><<<(unsigned)blocks, CT, 0, st>>>(a);
   else if (v == 4) commit_k<uint32_t><<<(unsigned)blocks, CT, 0, st>>>(a);
   else commit_k<uint16_t><<<(unsigned)blocks, CT, 0, st>>>(a);
-  return (int)cudaGetLastError();
+  return launched();
 }

@@ -377,7 +377,7 @@ struct KvAttnArgs {
   // scratch: 2 * ctas pieces of [rows, hd] and [rows, 2]; with weights [B, nkv, T * group, sp] scores
   // and [B, nkv, T * group, 2] maxima and inverse sums of the rows that no join sees
   float *part_o, *part_ml, *scores, *norm;
-  int* prefix;                        // [B + 1] tiles of one (head, row block) before every sequence
+  int* prefix;                        // [B + 1] costs of one (head, row block) before every sequence
   long sp;
   float inv_group;                    // 1 / group
   unsigned long long wait_ns;         // bound of the tcgen05 kernel's waits
@@ -389,6 +389,7 @@ int kv_attn_t5_launch(const KvAttnArgs& a, int dtype, cudaStream_t st);
 int kv_attn_tc_launch(const KvAttnArgs& a, int dtype, cudaStream_t st);
 void kv_attn_plan(KvAttnArgs& a, int dtype, int sms);
 int kv_attn_launch(const KvAttnArgs& a, int dtype, cudaStream_t st);
+long kv_launches();                    // kernels that the cache operators have launched so far
 int kv_status_word(int** word);        // the current device's word: 1 once a bounded wait of the tcgen05 kernel ran out
 
 // eviction from caches by accumulated weight (kv_evict.cu): N layers, B sequences, nkv heads
