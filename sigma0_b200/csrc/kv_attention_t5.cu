@@ -15,9 +15,8 @@
 // cp.async (rows past the end become 0, any strides), as far ahead as there are free slots.  Mbarriers
 // connect them; every wait is bounded: one that runs out ends all roles, makes the CTA's rows NaN and sets a status word.
 //
-// A unit costs some 8 tiles besides its own, and 20 at least (swept on 16 ragged contexts of up to 22,000 tokens
-// with 64 nodes: 529 us at 4 and 0, 385 us at 8 and 20): the trips for queries, mask bits and new rows take 3 us
-// each while the memory is busy, and only the tiles of a long unit cover them.
+// A unit costs some 8 tiles besides its own, and 20 at least (kv_attention.cuh has the sweep): the trips for queries, mask
+// bits and new rows take 3 us each while the memory is busy, and only the tiles of a long unit cover them.
 //
 // The softmax's reference moves only when a score passes it by far (see kv_attention_tc.cu); then
 // the rows' output in tensor memory is rescaled.  p is rounded once to the cache's type for the second product: a second
@@ -26,7 +25,7 @@
 // keys take less than the 64 KB of their K and V take from HBM (2,800 cycles of an SM at the copy rate):
 // the products read 6 KB of operands per 16-channel step from shared memory, some 770 cycles a tile; the
 // exponentials are 512 cycles of the SM's special function units.  Measured: 2,650-2,800 cycles a tile in a long unit;
-// 64 nodes over 16 contexts of up to 22,000 tokens, 16 heads of 128: 381 us with the join, 75% of the copy rate (500 us
+// 64 nodes over 16 contexts of up to 22,000 tokens, 16 heads of 128: 379 us with the join, 75% of the copy rate (500 us
 // for an mma.sync kernel with 64 rows, whose warps wait for one another's latencies at 44% of that pipe).
 #include <algorithm>
 

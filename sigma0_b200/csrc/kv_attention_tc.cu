@@ -16,7 +16,8 @@
 // running sum of its own and no barrier among warps; they are joined at the end of a unit.
 //
 // Measured: one token of 64 books over up to 11,000 cached ones, 16 heads of 64: 290-300 us, 97% of the copy rate
-// (with queries as the 16-row side: 430 us); one token over 66,000, 16 heads of 128: 84-87 us, the copy rate.
+// (with queries as the 16-row side: 430 us); one token over 66,000, 16 heads of 128: 84-87 us, the copy rate; without the
+// join in both.
 //
 // The maximum that the exponentials refer to moves only when a score passes it by 2^8 (2^4 in fp16, whose range is
 // short: see Ref in kv_attention.cuh): the probabilities may be that much larger, which changes no relative error, and

@@ -13,13 +13,13 @@
 // ranks, and the block moves its own rows, so that the selection of some units runs under the traffic of
 // others.  What bounds it is that traffic: 8 bytes read and written per slot and the moved rows.  With
 // fewer units than SMs a second kernel moves the rows instead, with several blocks per unit.  Measured: 11,000 -> 2,048
-// slots in 4 layers x 16 books x 16 heads of 64: 205 us, 70% of the copy rate; 4,118 -> 4,096 in 24 layers: 180 us (1,147
+// slots in 4 layers x 16 books x 16 heads of 64: 206 us, 70% of the copy rate; 4,118 -> 4,096 in 24 layers: 183 us (1,147
 // with serial digit searches and a scan per 512 slots), bound by the selection: 53% of the issue slots and its barriers.
 //
 // Acceptance.  The walk down a tree of drafted tokens takes the lowest child whose token is the
 // model's token after the node, until there is none; row len + path[j] moves to len + j.  Nodes whose rows lie past
 // the last slot were not stored, and the walk does not go to them.  A child
-// has a higher index than its parent, so path[j] >= j and rows can move upwards in order.  64 nodes, 24 layers x 32 books: 14.5 us, a chain of three
+// has a higher index than its parent, so path[j] >= j and rows can move upwards in order.  64 nodes, 24 layers x 32 books: 14.7 us, a chain of three
 // trips to memory (tree and lengths, rows, weights); the rows themselves are 5 us.
 #include <algorithm>
 
