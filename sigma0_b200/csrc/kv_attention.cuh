@@ -17,7 +17,7 @@
 // float32, one to 200 rows, contexts of up to 26,000.  Times in us at extra and least 0 and 0 / 8 and 16 / 8 and 20 /
 // 24 and 32: one token of 64 books 308 / 294 / 298 / 294, of 40 books of up to 1,500 tokens 69 / 50 / 48 / 50, a tree of 64
 // 579 / 368 / 345 / 349, 200 new tokens of 5 books 384 / 97 / 93 / 91, the float32 message 224 / 108 / 103 / 116.  From 8 on
-// it is flat, so that one pair serves all.
+// it is flat: 8 with 16 or 20 serves all.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

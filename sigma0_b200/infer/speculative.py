@@ -85,6 +85,8 @@ class TreeDecoder:
     def _need(self, new, nodes=0):
         """Raises where ``new`` tokens behind the cached ones do not fit, or a step of ``nodes`` beyond a budget that they reach."""
         c = self.caches[0]
+        if c.lengths.is_cuda and torch.cuda.is_current_stream_capturing():
+            return                                                        # nothing is known on the host
         rows = int(c.lengths.max()) + new
         if c.budget:
             rows = min(rows, c.budget + nodes)
@@ -94,7 +96,8 @@ class TreeDecoder:
     def prefill(self, tokens, book=None, chunk=512):
         """The prompt (B, L) in causal chunks that fit between budget and slots -> the model's next token (B,).
 
-        Without a budget the prompt must fit behind the cached tokens (reads their number on the host)."""
+        Without a budget the prompt must fit behind the cached tokens (their number is read on the host, but not in the
+        capture of a CUDA graph)."""
         c = self.caches[0]
         if not tokens.shape[1]:
             raise ValueError("a prompt of at least one token")

@@ -57,3 +57,30 @@ def test_a_budget_that_is_not_reached_needs_no_slots_beyond_it():
     model, prompt = _model(), _prompt(30)
     got, _ = generate(TreeDecoder(model, 3, 60, budget=58, recent=8), prompt, 20, width=2, depth=5)
     assert torch.equal(got, _greedy(model, prompt, 20))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("budget", [None, 40])
+def test_prefill_can_be_captured(budget):
+    """In a CUDA graph, where nothing can be read on the host: the replay does what the eager call does."""
+    model, prompt = _model().cuda(), _prompt(90).cuda()
+    runs = []
+    for graphed in (False, True):
+        dec = TreeDecoder(model, 3, 120, budget=budget, recent=8)
+        state = [x for c in dec.caches for x in (c.k, c.v, c.lengths, c.seen, c.weight, c.positions) if x is not None]
+        saved = [x.clone() for x in state]
+        st = torch.cuda.Stream()
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            token = dec.prefill(prompt, chunk=30)
+        torch.cuda.current_stream().wait_stream(st)
+        if graphed:
+            g = torch.cuda.CUDAGraph()
+            for x, y in zip(state, saved):
+                x.copy_(y)
+            with torch.cuda.graph(g):
+                token = dec.prefill(prompt, chunk=30)
+            g.replay()
+        torch.cuda.synchronize()
+        runs.append([token] + [x.clone() for x in state])
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
