@@ -939,7 +939,9 @@ std::vector<at::Tensor> kv_evict(at::Tensor kc, at::Tensor vc, at::Tensor weight
   kv_output(wo, weight, "weight");
   kv_output(po, positions, "positions");
   kv_output(lo, lengths, "lengths");
-  TORCH_CHECK(B == 0 || at::get_overlap_status(lo, seen) == at::MemOverlapStatus::No, "the lengths output must not be seen");
+  // lengths in place wait for all units, whatever else they are; others are written while units still read seen
+  TORCH_CHECK(B == 0 || lo.data_ptr() == lengths.data_ptr() || at::get_overlap_status(lo, seen) == at::MemOverlapStatus::No,
+              "the lengths output must not be seen");
   TORCH_CHECK((wo.data_ptr() != weight.data_ptr() || wo.strides() == weight.strides()) &&
                   (po.data_ptr() != positions.data_ptr() || po.strides() == positions.strides()),
               "an output that is its input must be the whole of it");

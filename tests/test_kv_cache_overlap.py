@@ -80,3 +80,14 @@ def test_outputs_across_their_inputs():
     both = torch.full((3,), 10, dtype=torch.int32, device="cuda")
     with pytest.raises(RuntimeError, match="overlaps"):
         cache_evict(kc, vc, w, pos, both[:2], seen, 4, out=(w, pos, both[1:]))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("nkv", [3, 300])
+def test_lengths_that_are_also_what_was_seen(dev, nkv):
+    """A first cut may be given one tensor for both, in place as well."""
+    kc, vc, w, pos, ls, _ = _case(dev, nkv=nkv)
+    k2, v2 = kc.clone(), vc.clone()
+    want = cache_evict(k2, v2, w, pos, ls.clone(), ls.clone(), 4, 2, 1)
+    got = cache_evict(kc, vc, w, pos, ls, ls, 4, 2, 1, out=(w, pos, ls))
+    assert got[2].tolist() == [4, 4] and all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(kc, k2) and torch.equal(vc, v2)
